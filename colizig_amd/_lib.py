@@ -56,6 +56,38 @@ class HbmPlan(ctypes.Structure):
     ]
 
 
+class KvCache(ctypes.Structure):
+    """`colizig_kv_cache`: one layer's paged cache."""
+
+    _fields_ = [
+        ("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp),
+        ("page_stride", ctypes.c_uint64), ("head_stride", ctypes.c_uint64), ("token_stride", ctypes.c_uint64),
+        ("pages", ctypes.c_uint32), ("page_size", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32), ("dtype", ctypes.c_uint32),
+    ]
+
+
+class AttnBatch(ctypes.Structure):
+    """`colizig_attn_batch`: the sequences of one attention call."""
+
+    _fields_ = [
+        ("row0", vp), ("len", vp), ("pages", vp),
+        ("n", ctypes.c_uint32), ("rows", ctypes.c_uint32), ("max_pages", ctypes.c_uint32),
+    ]
+
+
+class Rotation(ctypes.Structure):
+    """`colizig_rotation`: norm weights and rotation table of q and k."""
+
+    _fields_ = [
+        ("table", vp), ("q_norm", vp), ("k_norm", vp),
+        ("positions", ctypes.c_uint32), ("dims", ctypes.c_uint32), ("eps", ctypes.c_float),
+    ]
+
+
+_ATTEND = [ctypes.POINTER(KvCache), ctypes.POINTER(AttnBatch), ctypes.c_int, vp, ctypes.c_uint64, vp, ctypes.c_uint64,
+           ctypes.c_uint32, ctypes.c_float, vp, ctypes.c_uint64, vp]
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     # the existing backend ABI (src/backend/gpu.zig:20-34)
@@ -76,6 +108,14 @@ SIGNATURES = {
     "colizig_hip_stream_evict_all": (ctypes.c_int, []),
     "colizig_hip_matrix_load_bf16": (ctypes.c_int, [ctypes.c_uint64, vp, ctypes.c_int, ctypes.c_int]),
     "colizig_hip_matmul_bf16_dev": (ctypes.c_int, [vp, vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_uint64, vp]),
+    # attention between the projections
+    "colizig_hip_attn_append": (ctypes.c_int, [
+        ctypes.POINTER(KvCache), ctypes.POINTER(AttnBatch), ctypes.c_int, vp, ctypes.c_uint64, vp, ctypes.c_uint64, vp,
+        ctypes.c_uint64, vp, ctypes.c_uint64, ctypes.c_uint32, ctypes.POINTER(Rotation), vp]),
+    "colizig_hip_attn_decode": (ctypes.c_int, _ATTEND),
+    "colizig_hip_attn_prompt": (ctypes.c_int, _ATTEND),
+    "colizig_hip_attn_work_bytes": (ctypes.c_uint64, [ctypes.POINTER(KvCache), ctypes.POINTER(AttnBatch),
+                                                      ctypes.c_uint32]),
     # extensions
     "colizig_hip_dequant_fp8": (ctypes.c_int, [vp, vp, vp, ctypes.c_int, ctypes.c_int]),
     "colizig_hip_layer_init": (ctypes.c_int, [ctypes.c_uint32, ctypes.POINTER(Dims), vp]),

@@ -42,7 +42,7 @@ def _run(cmd: list[str]) -> None:
 def build_hip() -> str:
     tmp = HIP_LIB + ".tmp"
     _run([HIPCC, *HIP_FLAGS, "-I", os.path.join(ROOT, "include"), "-o", tmp,
-          os.path.join(CSRC, "colizig_hip.hip")])
+          os.path.join(CSRC, "colizig_hip.hip"), os.path.join(CSRC, "cz_attn.hip")])
     os.replace(tmp, HIP_LIB)
     return HIP_LIB
 

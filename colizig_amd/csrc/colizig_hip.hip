@@ -13,11 +13,13 @@
 #include "cz_sched.h"
 #include "cz_scratch.h"
 #include "cz_plan.h"
+#include "cz_attn.h"
 #include "colizig_hip.h"
 
 #include <xmmintrin.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -282,6 +284,8 @@ struct Ctx {
     int64_t next_handle = 1;
     StreamPool pool;
     FusedState fused;
+    uint32_t *attn_err_host = nullptr;  // host-coherent error words of the attention kernels
+    uint32_t *attn_err_dev = nullptr;   // their device address
     bool prefill_fp8 = true;   // grouped GEMMs on FP8 MFMA (k_gg8), else f16 (k_gg)
 };
 
@@ -1279,6 +1283,20 @@ int fused_check_error() {
     return -5;
 }
 
+// The attention kernels' error words (cz::AttnError), the same way.
+int attn_check_error() {
+    if (!g.attn_err_host) return 0;
+    uint32_t e[cz::kAttnErrors], any = 0;
+    for (uint32_t i = 0; i < cz::kAttnErrors; ++i)
+        any |= e[i] = __atomic_exchange_n(g.attn_err_host + i, 0u, __ATOMIC_ACQ_REL);
+    if (!any) return 0;
+    snprintf(g_err, sizeof g_err, "attention: %s%s%sthe results of that call are invalid",
+             e[cz::kAttnBadPage] ? "a page number outside the cache; " : "",
+             e[cz::kAttnBadLength] ? "rows or lengths outside rows and max_pages; " : "",
+             e[cz::kAttnBadPosition] ? "a position outside the rotation table; " : "");
+    return -5;
+}
+
 uint8_t *noalloc_scratch();
 
 // The one-launch decode's placement census (k_xcd_census): true when each of
@@ -1346,6 +1364,10 @@ extern "C" int colizig_cuda_init(void) {
     // the no-alloc forward's scratch address on this device; a failure is
     // reported by that entry point, which tries again
     if (!noalloc_scratch()) g_err[0] = 0;
+    if (hipHostMalloc(&g.attn_err_host, cz::kAttnErrors * sizeof(uint32_t), hipHostMallocCoherent) != hipSuccess ||
+        hipHostGetDevicePointer((void **)&g.attn_err_dev, g.attn_err_host, 0) != hipSuccess)
+        return -4;
+    memset(g.attn_err_host, 0, cz::kAttnErrors * sizeof(uint32_t));
     g.budget = 0;  // keyed cache off until set (colizig_cuda.cu:185)
     g.inited = 1;
     return 0;
@@ -1398,6 +1420,7 @@ extern "C" void colizig_cuda_shutdown(void) {
                     (void *)g.fused.hx, (void *)g.fused.run, (void *)g.fused.pred, (void *)g.fused.lgpx})
         if (p) (void)hipFree(p);
     if (g.fused.err_host) (void)hipHostFree(g.fused.err_host);
+    if (g.attn_err_host) (void)hipHostFree(g.attn_err_host);
     StreamPool &P = g.pool;
     if (P.copy) (void)hipStreamSynchronize(P.copy);
     if (P.copy_hi) (void)hipStreamSynchronize(P.copy_hi);
@@ -1808,6 +1831,193 @@ extern "C" int colizig_hip_matmul_fp8_dev_multi(int n, float *const *y_devs, con
         return -4;
     }
     return 0;
+}
+
+// ---- attention between the projections (cz_attn.hip) ------------------------
+namespace {
+
+// The library's device for the length of a call, whatever the caller's is.
+struct DeviceGuard {
+    int was = 0;
+    DeviceGuard() {
+        if (hipGetDevice(&was) == hipSuccess && was != 0) (void)hipSetDevice(0);
+    }
+    ~DeviceGuard() {
+        if (was != 0) (void)hipSetDevice(was);
+    }
+};
+
+bool attn_no(const char *why) {
+    snprintf(g_err, sizeof g_err, "attention: %s", why);
+    return false;
+}
+
+uint32_t attn_type_size(uint32_t t) { return t == COLIZIG_F32 ? 4 : t == COLIZIG_BF16 ? 2 : 1; }
+bool attn_mult16(uint64_t elements, uint32_t size) { return elements * size % 16 == 0; }
+
+// The sizes and types of a call: all that the scratch depends on.
+bool attn_sizes_ok(const colizig_kv_cache *c, const colizig_attn_batch *b, int dtype, uint32_t q_heads) {
+    if (!c || !b) return attn_no("no cache or no batch");
+    if (dtype != COLIZIG_F32 && dtype != COLIZIG_BF16) return attn_no("rows are f32 or BF16");
+    if (c->dtype > COLIZIG_E4M3 || (dtype == COLIZIG_BF16 && c->dtype == COLIZIG_F32))
+        return attn_no("caches are f32 (f32 rows alone), BF16 or E4M3");
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return attn_no("head_dim is 64, 128 or 256");
+    if (!c->page_size || c->page_size % 16) return attn_no("page_size is a multiple of 16");
+    if (!c->pages || c->pages > 0x7fffffffu) return attn_no("pages outside 1 .. 2^31 - 1");
+    if (!c->kv_heads || q_heads % c->kv_heads || q_heads > 65535 || c->kv_heads > 65535)
+        return attn_no("q_heads is a multiple of kv_heads, both at most 65535");
+    if (!b->n || !b->rows || !b->max_pages) return attn_no("n, rows and max_pages are at least 1");
+    if (!b->row0 && b->rows != b->n) return attn_no("without row0 there is one row per sequence");
+    if (b->n > 0xffffffu || (uint64_t)b->rows * (q_heads + 2 * c->kv_heads) > 0x7fffffffu)
+        return attn_no("too many sequences or rows for one call");
+    if ((uint64_t)b->max_pages * c->page_size > 0x7fffffffu) return attn_no("max_pages * page_size over 2^31 - 1");
+    return true;
+}
+
+bool attn_rows_ok(const void *p, uint64_t *stride, uint64_t width, int dtype) {
+    if (!p) return attn_no("a row tensor is missing");
+    if ((uintptr_t)p & 15u) return attn_no("row tensors must be 16-byte aligned");
+    if (!*stride) *stride = width;
+    if (*stride < width || *stride > (1ull << 40) || !attn_mult16(*stride, attn_type_size(dtype)))
+        return attn_no("a row stride is at least the row's heads and of whole 16 bytes");
+    return true;
+}
+
+bool attn_cache_args(const colizig_kv_cache *c, const colizig_attn_batch *b, cz::AttnCache *o) {
+    const uint32_t size = attn_type_size(c->dtype);
+    if (!c->k || !c->v || !b->len || !b->pages) return attn_no("a null pointer in the cache or the batch");
+    if ((((uintptr_t)c->k) | ((uintptr_t)c->v)) & 15u) return attn_no("k and v must be 16-byte aligned");
+    if ((((uintptr_t)b->len) | ((uintptr_t)b->pages) | ((uintptr_t)b->row0) | ((uintptr_t)c->k_scale) |
+         ((uintptr_t)c->v_scale)) & 3u)
+        return attn_no("lengths, pages, row0 and scales must be 4-byte aligned");
+    uint64_t ts = c->token_stride, hs = c->head_stride, ps = c->page_stride;
+    if (!ts && !hs && !ps) {
+        ts = c->head_dim;
+        hs = (uint64_t)c->page_size * ts;
+        ps = c->kv_heads * hs;
+    }
+    if (ts < c->head_dim || (c->kv_heads > 1 && hs < c->head_dim) || (c->pages > 1 && ps < c->head_dim) ||
+        (ts | hs | ps) > (1ull << 40) || !attn_mult16(ts, size) || !attn_mult16(hs, size) || !attn_mult16(ps, size))
+        return attn_no("a cache stride is at least head_dim and of whole 16 bytes");
+    *o = cz::AttnCache{c->k,      c->v,         c->k_scale,  c->v_scale, ps,      hs,      ts, c->pages, c->page_size,
+                       c->kv_heads, c->dtype, b->row0, b->len,    b->pages, b->n, b->rows, b->max_pages, g.attn_err_dev};
+    return true;
+}
+
+int attn_launched(const char *what) {
+    const hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return 0;
+    snprintf(g_err, sizeof g_err, "%s launch: %s", what, hipGetErrorString(e));
+    return -4;
+}
+
+int attn_run(const char *what, const colizig_kv_cache *cache, const colizig_attn_batch *batch, int dtype,
+             const void *q, uint64_t q_stride, void *out, uint64_t out_stride, uint32_t q_heads, float scale,
+             void *work, uint64_t work_bytes, void *stream) {
+    if (!g.inited) return attn_no("the library is not initialised"), -1;
+    cz::AttnArgs A{};
+    if (!q_heads || !std::isfinite(scale)) return attn_no("q_heads is at least 1 and scale finite"), -1;
+    const uint64_t width = (uint64_t)q_heads * cache->head_dim;
+    if (!attn_cache_args(cache, batch, &A.c) || !attn_rows_ok(q, &q_stride, width, dtype) ||
+        !attn_rows_ok(out, &out_stride, width, dtype))
+        return -1;
+    A.q = q;
+    A.out = out;
+    A.q_stride = q_stride;
+    A.out_stride = out_stride;
+    A.group = q_heads / cache->kv_heads;
+    A.scale = scale;
+    A.work = work;
+    if (!work || ((uintptr_t)work & 15u) || work_bytes < cz::attn_work_bytes(A, cache->head_dim))
+        return attn_no("scratch missing, not 16-byte aligned or under colizig_hip_attn_work_bytes"), -1;
+    DeviceGuard dev;
+    cz::launch_attn(A, dtype, cache->head_dim, pick_stream(stream));
+    return attn_launched(what);
+}
+
+}  // namespace
+
+extern "C" int colizig_hip_attn_append(const colizig_kv_cache *cache, const colizig_attn_batch *batch, int dtype,
+                                       const void *q, uint64_t q_stride, const void *k, uint64_t k_stride,
+                                       const void *v, uint64_t v_stride, void *q_out, uint64_t q_out_stride,
+                                       uint32_t q_heads, const colizig_rotation *rotation, void *stream) {
+    CsrGuard csr;
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (!attn_sizes_ok(cache, batch, dtype, q_heads)) return -1;
+    cz::AppendArgs A{};
+    const uint64_t dim = cache->head_dim;
+    if (!q != !q_out || (q && !q_heads)) return attn_no("q and q_out come together, with q_heads"), -1;
+    if (!attn_cache_args(cache, batch, &A.c) || !attn_rows_ok(k, &k_stride, cache->kv_heads * dim, dtype) ||
+        !attn_rows_ok(v, &v_stride, cache->kv_heads * dim, dtype) ||
+        (q && (!attn_rows_ok(q, &q_stride, q_heads * dim, dtype) ||
+               !attn_rows_ok(q_out, &q_out_stride, q_heads * dim, dtype))))
+        return -1;
+    if (rotation) {
+        const colizig_rotation &R = *rotation;
+        if ((((uintptr_t)R.table) | ((uintptr_t)R.q_norm) | ((uintptr_t)R.k_norm)) & 15u)
+            return attn_no("the rotation's arrays must be 16-byte aligned"), -1;
+        if (R.table && (!R.positions || !R.dims || R.dims % 16 || R.dims > dim))
+            return attn_no("a rotation has positions, and dims a multiple of 16 up to head_dim"), -1;
+        if ((R.q_norm || R.k_norm) && !(R.eps >= 0.0f && std::isfinite(R.eps)))
+            return attn_no("eps is finite and not negative"), -1;
+        A.rope = R.table;
+        A.positions = R.positions;
+        A.dims = R.dims;
+        A.q_norm = R.q_norm;
+        A.k_norm = R.k_norm;
+        A.eps = R.eps;
+    }
+    if (!g.inited) return attn_no("the library is not initialised"), -1;
+    A.q = q;
+    A.k = k;
+    A.v = v;
+    A.q_out = q_out;
+    A.q_stride = q_stride;
+    A.k_stride = k_stride;
+    A.v_stride = v_stride;
+    A.q_out_stride = q_out_stride;
+    A.q_heads = q ? q_heads : 0;
+    DeviceGuard dev;
+    cz::launch_append(A, dtype, cache->head_dim, pick_stream(stream));
+    return attn_launched("attn_append");
+}
+
+extern "C" int colizig_hip_attn_decode(const colizig_kv_cache *cache, const colizig_attn_batch *batch, int dtype,
+                                       const void *q, uint64_t q_stride, void *out, uint64_t out_stride,
+                                       uint32_t q_heads, float scale, void *work, uint64_t work_bytes, void *stream) {
+    CsrGuard csr;
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (!attn_sizes_ok(cache, batch, dtype, q_heads)) return -1;
+    if (batch->row0) return attn_no("one token per sequence takes no row0"), -1;
+    return attn_run("attn_decode", cache, batch, dtype, q, q_stride, out, out_stride, q_heads, scale, work, work_bytes,
+                    stream);
+}
+
+extern "C" int colizig_hip_attn_prompt(const colizig_kv_cache *cache, const colizig_attn_batch *batch, int dtype,
+                                       const void *q, uint64_t q_stride, void *out, uint64_t out_stride,
+                                       uint32_t q_heads, float scale, void *work, uint64_t work_bytes, void *stream) {
+    CsrGuard csr;
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (!attn_sizes_ok(cache, batch, dtype, q_heads)) return -1;
+    if (!batch->row0) return attn_no("a prompt needs row0"), -1;
+    return attn_run("attn_prompt", cache, batch, dtype, q, q_stride, out, out_stride, q_heads, scale, work, work_bytes,
+                    stream);
+}
+
+extern "C" uint64_t colizig_hip_attn_work_bytes(const colizig_kv_cache *cache, const colizig_attn_batch *batch,
+                                                uint32_t q_heads) {
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (!attn_sizes_ok(cache, batch, COLIZIG_F32, q_heads) || !q_heads) return 0;
+    cz::AttnArgs A{};
+    A.c.kv_heads = cache->kv_heads;
+    A.c.dtype = cache->dtype;
+    A.c.page_size = cache->page_size;
+    A.c.row0 = batch->row0;
+    A.c.n = batch->n;
+    A.c.rows = batch->rows;
+    A.c.max_pages = batch->max_pages;
+    A.group = q_heads / cache->kv_heads;
+    return cz::attn_work_bytes(A, cache->head_dim);
 }
 
 // ===========================================================================
@@ -4005,7 +4215,8 @@ extern "C" int colizig_hip_sync(void) {
     CsrGuard csr;
     if (!g.inited) return -1;
     CZ_CHECK(hipStreamSynchronize(g.stream), -5);
-    return fused_check_error();
+    const int rc = fused_check_error();
+    return rc ? rc : attn_check_error();
 }
 extern "C" int64_t colizig_hip_event_create(void) {
     CsrGuard csr;

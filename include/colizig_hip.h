@@ -106,6 +106,109 @@ int colizig_hip_matmul_fp8_dev_multi(int n, float *const *y_devs, const uint64_t
 int colizig_hip_matrix_load_bf16(uint64_t key, const uint16_t *w, int I, int O);
 int colizig_hip_matmul_bf16_dev(float *y_dev, const float *x_dev, int S, int I, int O, uint64_t key, void *stream);
 
+/* ---- attention between the projections -----------------------------------
+ * What a caller with device activations needs between the q, k, v and o
+ * projections above (src/qwen3moe/attn.zig:209-259 on the engine's CPU): new
+ * keys and values into a paged cache, one new token per sequence attending
+ * over it, and prompts.  Everything is on device pointers and asynchronous on
+ * `stream` (NULL = the library's stream); nothing is allocated, so every call
+ * can be captured into a graph.
+ *
+ * Types of rows (q, k, v, out) and caches.  f32 rows go with every cache,
+ * BF16 rows with BF16 and E4M3 caches. */
+#define COLIZIG_F32 0
+#define COLIZIG_BF16 1
+#define COLIZIG_E4M3 2
+
+/* One layer's paged cache.  A page holds page_size tokens of every key head;
+ * element d of token slot s of head h in page p is at p*page_stride +
+ * h*head_stride + s*token_stride + d (strides in elements, of whole 16 bytes;
+ * all three 0: [page][head][slot][dim]).  k and v have the same layout and are
+ * 16-byte aligned.  page_size is a multiple of 16, head_dim 64, 128 or 256.
+ * An E4M3 cache holds value / scale, one f32 scale per key head (NULL: 1);
+ * the other types ignore the scales. */
+typedef struct colizig_kv_cache {
+    void *k, *v;
+    const float *k_scale, *v_scale; /* device [kv_heads] */
+    uint64_t page_stride, head_stride, token_stride;
+    uint32_t pages, page_size, kv_heads, head_dim;
+    uint32_t dtype;
+} colizig_kv_cache;
+
+/* The sequences of one call.  Sequence b's new tokens are rows row0[b] ..
+ * row0[b + 1] - 1 of the row tensors (row0 NULL: row b alone, and rows = n);
+ * len[b] tokens of it are in the cache, the new ones last: new token i sits at
+ * position len[b] - (row0[b + 1] - row0[b]) + i and sees the positions up to
+ * its own.  pages[b * max_pages + j] is the cache page of its positions
+ * j*page_size ... .  A row at a negative position is padding: it is not
+ * appended, its query is not written, and as an attention row it gives zeros.
+ * Rows behind row0[n] are not read or written.  All three arrays are device
+ * memory and read when the work runs, so a captured call follows them.
+ * What they hold is checked there: a page number outside the cache (not
+ * written, read as page 0), rows or lengths outside rows and max_pages (cut),
+ * and a position outside the rotation's table (not appended) make the next
+ * colizig_hip_sync return -5 with a message; the call's results are then
+ * invalid, and no access is out of bounds. */
+typedef struct colizig_attn_batch {
+    const int32_t *row0;  /* [n + 1] or NULL */
+    const int32_t *len;   /* [n] */
+    const int32_t *pages; /* [n][max_pages] */
+    uint32_t n, rows, max_pages;
+} colizig_attn_batch;
+
+/* What happens to q and k on the way: RMS norm per head, x / sqrt(mean(x^2) +
+ * eps) * weight (q_norm, k_norm: f32 [head_dim]; NULL: none), then the first
+ * `dims` numbers turned by the position, number d with number d + dims/2.
+ * table: f32 [positions][dims], a position's dims/2 cosines, then its sines
+ * (NULL: no rotation).  dims is even, a multiple of 16, at most head_dim. */
+typedef struct colizig_rotation {
+    const float *table;
+    const float *q_norm, *k_norm;
+    uint32_t positions, dims;
+    float eps;
+} colizig_rotation;
+
+/* Puts the new tokens' keys and values into the cache, rounded once to its
+ * type (E4M3: saturating at 448 scales), and the normalised and rotated
+ * queries into q_out (which may be q; q and q_out NULL: keys and values
+ * only).  rows of dtype COLIZIG_F32 or COLIZIG_BF16; a row's heads are
+ * contiguous, strides (elements; 0 = dense) are from row to row, so a fused
+ * q|k|v row serves.  Pointers 16-byte aligned, strides of whole 16 bytes.
+ * rotation NULL: neither norm nor rotation.  The caller keeps two sequences
+ * from sharing a page that is written.  0, -1 bad arguments, -4 launch. */
+int colizig_hip_attn_append(const colizig_kv_cache *cache, const colizig_attn_batch *batch, int dtype, const void *q,
+                            uint64_t q_stride, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride,
+                            void *q_out, uint64_t q_out_stride, uint32_t q_heads, const colizig_rotation *rotation,
+                            void *stream);
+
+/* Attention of one new token per sequence (batch->row0 NULL):
+ *   out[b][x] = sum_j softmax_j(scale * q[b][x] . k_j) v_j,  j < len[b],
+ * with the keys and values of head x / (q_heads / kv_heads).  A sequence of
+ * length 0 gives zeros.  Products and sums of f32 rows are at f32 accuracy;
+ * for BF16 rows the softmax weights are rounded to BF16 for their products,
+ * and the result once.  out may be q.  work: device scratch of
+ * colizig_hip_attn_work_bytes, 16-byte aligned, held by no other call that
+ * may run at the same time (a captured graph's stays its own); its contents
+ * mean nothing between calls.  A row's bits depend on how the lengths of the
+ * batch divide the work, not on other rows' values.  0, -1 bad arguments or
+ * too little scratch, -4 launch. */
+int colizig_hip_attn_decode(const colizig_kv_cache *cache, const colizig_attn_batch *batch, int dtype, const void *q,
+                            uint64_t q_stride, void *out, uint64_t out_stride, uint32_t q_heads, float scale,
+                            void *work, uint64_t work_bytes, void *stream);
+
+/* The same for sequences of any number of new tokens (batch->row0 given): a
+ * whole prompt (len = its tokens), a chunk of one or a draft on top of cached
+ * tokens, several of them packed.  The keys and values of the new tokens are
+ * in the cache already.  Arguments and results as for one token. */
+int colizig_hip_attn_prompt(const colizig_kv_cache *cache, const colizig_attn_batch *batch, int dtype, const void *q,
+                            uint64_t q_stride, void *out, uint64_t out_stride, uint32_t q_heads, float scale,
+                            void *work, uint64_t work_bytes, void *stream);
+
+/* Scratch of an attention call with this cache, batch and head count: looks at
+ * sizes alone (n, rows, max_pages, whether row0 is given), reads no device
+ * memory and needs no device.  0 where the call would be refused. */
+uint64_t colizig_hip_attn_work_bytes(const colizig_kv_cache *cache, const colizig_attn_batch *batch, uint32_t q_heads);
+
 /* ------------------------------------------------------------------------ */
 /* 2. MoE-level extensions                                                   */
 /* ------------------------------------------------------------------------ */
