@@ -1897,8 +1897,8 @@ bool attn_cache_args(const colizig_kv_cache *c, const colizig_attn_batch *b, cz:
         ps = c->kv_heads * hs;
     }
     if (ts < c->head_dim || (c->kv_heads > 1 && hs < c->head_dim) || (c->pages > 1 && ps < c->head_dim) ||
-        (ts | hs | ps) > (1ull << 40) || !attn_mult16(ts, size) || !attn_mult16(hs, size) || !attn_mult16(ps, size))
-        return attn_no("a cache stride is at least head_dim and of whole 16 bytes");
+        ts > (1ull << 24) || hs > (1ull << 40) || ps > (1ull << 40) || (double)c->pages * (double)ps > 0x1p60 || !attn_mult16(ts, size) || !attn_mult16(hs, size) || !attn_mult16(ps, size))
+        return attn_no("a cache stride is at least head_dim, of whole 16 bytes and not over 2^24 (token), 2^40 elements");
     *o = cz::AttnCache{c->k,      c->v,         c->k_scale,  c->v_scale, ps,      hs,      ts, c->pages, c->page_size,
                        c->kv_heads, c->dtype, b->row0, b->len,    b->pages, b->n, b->rows, b->max_pages, g.attn_err_dev};
     return true;

@@ -108,7 +108,8 @@ def test_not_initialised_is_refused():
 @pytest.mark.parametrize("kw,why", [
     (dict(c=cache(k_ptr=None)), "null"), (dict(c=cache(v_ptr=A + 8)), "aligned"),
     (dict(c=cache(strides=(0, 0, 64))), "stride"), (dict(c=cache(strides=(8192, 2048, 132))), "stride"),
-    (dict(c=cache(strides=(0, 2048, 128))), "stride"),
+    (dict(c=cache(strides=(0, 2048, 128))), "stride"), (dict(c=cache(strides=(8192, 2048, (1 << 24) + 128))), "stride"),
+    (dict(c=cache(strides=(1 << 41, 2048, 128))), "stride"),
     (dict(b=batch(len_ptr=None)), "null"), (dict(b=batch(pages_ptr=None)), "null"), (dict(b=batch(len_ptr=A + 2)), "aligned"),
     (dict(q=None), "missing"), (dict(out=A + 4), "aligned"), (dict(sq=32 * 128 - 4), "stride"),
     (dict(so=32 * 128 + 2), "stride"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
