@@ -17,33 +17,15 @@ __device__ __forceinline__ void flag(uint32_t *err, AttnError what) {
     __hip_atomic_store(err + what, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
-__device__ __forceinline__ uint16_t bf16_rne(float x) {
-    const __bf16 b = (__bf16)x;
-    uint16_t u;
-    __builtin_memcpy(&u, &b, 2);
-    return u;
-}
-__device__ __forceinline__ float bf16_f32(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
-
-// Nearest E4M3 byte (ties to even), saturating at 448; a NaN stays one.
-__device__ __forceinline__ uint8_t e4m3_rne(float x) {
-    const float c = x != x ? x : fminf(fmaxf(x, -448.0f), 448.0f);
-    return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(c, c, 0, false) & 255);
-}
+// What saturates to an E4M3 number: rounding to nearest follows.  A NaN stays one.
+__device__ __forceinline__ float e4m3_range(float x) { return x != x ? x : fminf(fmaxf(x, -448.0f), 448.0f); }
 
 template <uint32_t T>
 __device__ __forceinline__ float load1(const void *p, uint64_t i) {
     if constexpr (T == kF32) return ((const float *)p)[i];
-    if constexpr (T == kBF16) return bf16_f32(((const uint16_t *)p)[i]);
+    if constexpr (T == kBF16) return __uint_as_float((uint32_t)((const uint16_t *)p)[i] << 16);
     if constexpr (T == kE4M3) return __builtin_amdgcn_cvt_f32_fp8(((const uint8_t *)p)[i], 0);
 }
-template <uint32_t T>
-__device__ __forceinline__ void store1(void *p, uint64_t i, float x) {
-    if constexpr (T == kF32) ((float *)p)[i] = x;
-    if constexpr (T == kBF16) ((uint16_t *)p)[i] = bf16_rne(x);
-    if constexpr (T == kE4M3) ((uint8_t *)p)[i] = e4m3_rne(x);
-}
-
 // Rows and length of sequence b, checked: 0 <= r0 <= r1 <= rows, 0 <= len <=
 // max_pages * page_size.  What is outside is flagged and cut.
 struct Seq {
@@ -65,17 +47,6 @@ __device__ __forceinline__ Seq sequence(const AttnCache &c, uint32_t b) {
     return s;
 }
 
-// The sequence of a row, or n where the row belongs to none.
-__device__ __forceinline__ uint32_t sequence_of(const AttnCache &c, uint32_t row) {
-    if (!c.row0) return row;
-    uint32_t lo = 0, hi = c.n;  // first b with row0[b + 1] > row
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (c.row0[mid + 1] > (int32_t)row) hi = mid; else lo = mid + 1;
-    }
-    return lo;
-}
-
 // A page number of the table; one outside the cache is flagged and read as 0.
 __device__ __forceinline__ uint32_t page_at(const AttnCache &c, uint32_t b, uint32_t i) {
     // uniform: a scalar load
@@ -85,80 +56,6 @@ __device__ __forceinline__ uint32_t page_at(const AttnCache &c, uint32_t b, uint
     return 0;
 }
 
-// ---- append -------------------------------------------------------------------
-// A wave per head vector: head x of row t, of the query (rotated into q_out),
-// then the keys, then the values.  A pair of the rotation sits in one lane.
-template <uint32_t R, uint32_t C, int D>
-__global__ __launch_bounds__(256) void k_append(AppendArgs A) {
-    constexpr int N = D / 64;
-    const uint32_t lane = threadIdx.x & 63, heads = A.q_heads + 2 * A.c.kv_heads;
-    const uint64_t item = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    const uint32_t t = (uint32_t)(item / heads), x = (uint32_t)(item % heads);
-    if (t >= A.c.rows) return;
-    const uint32_t b = sequence_of(A.c, t);
-    if (b >= A.c.n) return;
-    const Seq s = sequence(A.c, b);
-    const int32_t pos = s.len - s.nq + ((int32_t)t - s.r0);
-    if (pos < 0) return;
-    const uint32_t kind = x < A.q_heads ? 0 : x < A.q_heads + A.c.kv_heads ? 1 : 2;
-    const uint32_t h = kind == 0 ? x : kind == 1 ? x - A.q_heads : x - A.q_heads - A.c.kv_heads;
-    const void *src = kind == 0 ? A.q : kind == 1 ? A.k : A.v;
-    const uint64_t at = (uint64_t)t * (kind == 0 ? A.q_stride : kind == 1 ? A.k_stride : A.v_stride) + (uint64_t)h * D;
-    if (kind != 2 && A.rope && (uint32_t)pos >= A.positions) {
-        flag(A.c.err, kAttnBadPosition);
-        return;
-    }
-    float y[N];
-    const float *w = kind == 0 ? A.q_norm : kind == 1 ? A.k_norm : nullptr;
-    float ss = 0;
-    for (int i = 0; i < N; ++i) {
-        y[i] = load1<R>(src, at + i * 64 + lane);
-        ss = __builtin_fmaf(y[i], y[i], ss);
-    }
-    if (w) {
-        for (int m = 32; m; m >>= 1) ss += __shfl_xor(ss, m);
-        const float r = 1.0f / __builtin_sqrtf(ss / D + A.eps);
-        for (int i = 0; i < N; ++i) y[i] = y[i] * r * w[i * 64 + lane];
-    }
-    __shared__ float sh[4][D];
-    float *mine = sh[threadIdx.x / 64];
-    if (kind != 2 && A.rope) {
-        for (int i = 0; i < N; ++i) mine[i * 64 + lane] = y[i];
-        __builtin_amdgcn_wave_barrier();
-        const float *cs = A.rope + (uint64_t)pos * A.dims;
-        const uint32_t half = A.dims / 2;
-        for (int i = 0; i < N; ++i) {
-            const uint32_t d = i * 64 + lane;
-            if (d < half) y[i] = mine[d] * cs[d] - mine[d + half] * cs[half + d];
-            else if (d < A.dims) y[i] = mine[d] * cs[d - half] + mine[d - half] * cs[d];
-        }
-    }
-    if (kind == 0) {
-        for (int i = 0; i < N; ++i) store1<R>(A.q_out, (uint64_t)t * A.q_out_stride + (uint64_t)h * D + i * 64 + lane, y[i]);
-        return;
-    }
-    const uint32_t page = (uint32_t)A.c.table[(uint64_t)b * A.c.max_pages + pos / A.c.page_size];
-    if (page >= A.c.pages) {
-        flag(A.c.err, kAttnBadPage);
-        return;
-    }
-    const uint64_t to = page * A.c.page_stride + h * A.c.head_stride + (pos % A.c.page_size) * A.c.token_stride;
-    const float *sc = kind == 1 ? A.c.k_scale : A.c.v_scale;
-    for (int i = 0; i < N; ++i) {
-        const float z = C == kE4M3 && sc ? y[i] / sc[h] : y[i];
-        store1<C>(kind == 1 ? A.c.k : A.c.v, to + i * 64 + lane, z);
-    }
-}
-
-// ---- attention ------------------------------------------------------------------
-// Rows of a key head: row r of a sequence's tile list is token r / group, query
-// head h * group + r % group, so the query heads of a key head share its loads.
-//
-// Both kernels work on S^T = K Q^T and O^T = V^T P^T: the scores' result layout
-// (a lane holds one row and 4 keys in a run) is the second product's operand
-// layout once its keys are counted in that order, so weights go from one matrix
-// instruction to the next in registers; V's side of it, 4 keys of one number, is
-// what the transposing LDS read gives.
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -222,13 +119,16 @@ struct Eight<kF32> {
         b = *(const u32x4 *)(p + 16);
     }
     __device__ __forceinline__ void zero() { a = b = u32x4{0, 0, 0, 0}; }
-    __device__ __forceinline__ void terms(bf8 (&t)[3]) const {
-        float x[8];
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             x[i] = __uint_as_float(a[i]);
             x[4 + i] = __uint_as_float(b[i]);
         }
+    }
+    __device__ __forceinline__ void terms(bf8 (&t)[3]) const {
+        float x[8];
+        floats(x);
         split8<3>(x, t);
     }
 };
@@ -237,6 +137,13 @@ struct Eight<kBF16> {
     u32x4 a;
     __device__ __forceinline__ void load(const uint8_t *p) { a = *(const u32x4 *)p; }
     __device__ __forceinline__ void zero() { a = u32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(a[i] << 16);
+            x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+        }
+    }
     __device__ __forceinline__ void terms(bf8 (&t)[1]) const { t[0] = __builtin_bit_cast(bf8, a); }
 };
 template <>
@@ -247,6 +154,237 @@ struct Eight<kE4M3> {
     __device__ __forceinline__ void terms(bf8 (&t)[1]) const { t[0] = e4m3x8(a[0], a[1]); }
 };
 
+// threadIdx.x as a value that the compiler knows nothing of: what rare or final code
+// derives from it is worked out there, not held in registers through the loops.
+__device__ __forceinline__ uint32_t thread_id() {
+    uint32_t t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
+// Numbers of type T in a word that are not finite become 0; whether there were any.
+template <uint32_t T>
+__device__ __forceinline__ bool clean(uint32_t &w) {
+    uint32_t bad;
+    if constexpr (T == kF32) {
+        bad = (w & 0x7f800000u) == 0x7f800000u ? ~0u : 0u;
+    } else if constexpr (T == kBF16) {
+        bad = ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+    } else {
+        // 0x7f and 0xff: the sum carries into the sign bit where the low bits are all set
+        bad = ((w & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u) >> 7;
+        bad *= 0xffu;
+    }
+    w &= ~bad;
+    return bad != 0;
+}
+
+// What a lane loads at a time: 8 numbers, of an E4M3 cache 16 so that it is 16 bytes.
+template <uint32_t T>
+struct Piece {
+    static constexpr int N = 8;
+    Eight<T> e;
+    __device__ __forceinline__ void load(const uint8_t *p) { e.load(p); }
+    __device__ __forceinline__ void zero() { e.zero(); }
+    __device__ __forceinline__ bool clean() {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w = e.a[i];
+            any |= cz::clean<T>(w);
+            e.a[i] = w;
+            if constexpr (T == kF32) {
+                w = e.b[i];
+                any |= cz::clean<T>(w);
+                e.b[i] = w;
+            }
+        }
+        return any;
+    }
+    __device__ __forceinline__ void terms(int, bf8 (&t)[kTerms<T>]) const { e.terms(t); }
+};
+template <>
+struct Piece<kE4M3> {
+    static constexpr int N = 16;
+    u32x4 a;
+    __device__ __forceinline__ void load(const uint8_t *p) { a = *(const u32x4 *)p; }
+    __device__ __forceinline__ void zero() { a = u32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ bool clean() {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w = a[i];
+            any |= cz::clean<kE4M3>(w);
+            a[i] = w;
+        }
+        return any;
+    }
+    __device__ __forceinline__ void terms(int half, bf8 (&t)[1]) const { t[0] = e4m3x8(a[2 * half], a[2 * half + 1]); }
+};
+
+// 8 numbers rounded to type T, 16-byte aligned (E4M3: 8).
+template <uint32_t T>
+__device__ __forceinline__ void store8(uint8_t *p, const float (&y)[8]) {
+    if constexpr (T == kF32) {
+        *(f32x4 *)p = f32x4{y[0], y[1], y[2], y[3]};
+        *(f32x4 *)(p + 16) = f32x4{y[4], y[5], y[6], y[7]};
+    } else if constexpr (T == kBF16) {
+        bf8 v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (__bf16)y[i];
+        *(bf8 *)p = v;
+    } else {
+        u32x2 w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float *x = y + 4 * i;
+            int v = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_range(x[0]), e4m3_range(x[1]), 0, false);
+            w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_range(x[2]), e4m3_range(x[3]), v, true);
+        }
+        *(u32x2 *)p = w;
+    }
+}
+
+// ---- append -------------------------------------------------------------------
+// Head vectors (the query's into q_out, then the keys, then the values) over groups
+// of D / 8 lanes, 8 neighbouring numbers a lane, so that a vector moves in 16-byte
+// pieces.  A norm's sum goes over the group's lanes; a rotation's other half is
+// dims / 16 lanes away.  A workgroup takes TB rows: the three lookups one after the
+// other (sequence, length, page and angles) cost it some microseconds whatever it
+// moves, and a group's angles and weights serve all its vectors of the row.
+// Few rows are spread over blockIdx.y too.
+template <uint32_t R, uint32_t C, int D, int TB>
+__global__ __launch_bounds__(256) void k_append(AppendArgs A) {
+    constexpr uint32_t LV = D / 8, GROUPS = 256 / LV, STEP = GROUPS / TB, UNROLL = TB == 1 ? 1 : 4;
+    const uint32_t lane = threadIdx.x & 63, gl = threadIdx.x % LV, gv = threadIdx.x / LV;
+    const uint32_t heads = A.q_heads + 2 * A.c.kv_heads, t0 = blockIdx.x * TB, t = t0 + gv % TB;
+    const uint32_t xs = gv / TB + blockIdx.y * STEP, xstep = STEP * gridDim.y;
+    Eight<R> in[UNROLL];
+    auto load = [&](uint32_t x0) {
+#pragma unroll
+        for (uint32_t u = 0; u < UNROLL; ++u) {
+            const uint32_t x = x0 + u * xstep;
+            in[u].zero();
+            if (x >= heads || t >= A.c.rows) continue;
+            const bool isq = x < A.q_heads, isk = x < A.q_heads + A.c.kv_heads;
+            const uint32_t h = isq ? x : isk ? x - A.q_heads : x - A.q_heads - A.c.kv_heads;
+            const uint64_t at = (uint64_t)t * (isq ? A.q_stride : isk ? A.k_stride : A.v_stride) + h * D + gl * 8;
+            in[u].load((const uint8_t *)(isq ? A.q : isk ? A.k : A.v) + at * kSize<R>);
+        }
+    };
+    load(xs);
+    // the row's sequence: as many as end at or before it
+    uint32_t b = 0;
+    if (A.c.row0) {
+        for (uint32_t b0 = 0; b0 < A.c.n; b0 += 64) {
+            const int32_t e = b0 + lane < A.c.n ? A.c.row0[b0 + lane + 1] : 0x7fffffff;
+#pragma unroll
+            for (uint32_t i = 0; i < TB; ++i) {
+                const uint32_t k = __popcll(__ballot(e <= (int32_t)(t0 + i)));
+                b += gv % TB == i ? k : 0;
+            }
+        }
+    } else {
+        b = t;
+    }
+    Seq s{0, 0, 0};
+    if (b < A.c.n && t < A.c.rows) s = sequence(A.c, b);
+    const int32_t pos = s.len - s.nq + ((int32_t)t - s.r0);
+    bool here = pos >= 0 && (int32_t)t >= s.r0 && (int32_t)t < s.r0 + s.nq;
+    if (here && A.rope && (uint32_t)pos >= A.positions) {
+        flag(A.c.err, kAttnBadPosition);
+        here = false;
+    }
+    bool paged = false;
+    uint64_t to = 0;
+    const uint32_t half = A.dims / 2, d0 = gl * 8;
+    const bool turns = A.rope && d0 < A.dims, lower = d0 < half;
+    float cs[8], sn[8], wq[8], wk[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        cs[i] = wq[i] = wk[i] = 1.0f;
+        sn[i] = 0.0f;
+    }
+    if (here) {
+        const uint32_t pi = (uint32_t)pos / A.c.page_size, page = (uint32_t)A.c.table[(uint64_t)b * A.c.max_pages + pi];
+        // the lane's angles: numbers d < dims/2 turn with d + dims/2
+        if (turns) {
+            const float *p = A.rope + (uint64_t)pos * A.dims + (lower ? d0 : d0 - half);
+            *(f32x4 *)cs = *(const f32x4 *)p;
+            *(f32x4 *)(cs + 4) = *(const f32x4 *)(p + 4);
+            *(f32x4 *)sn = *(const f32x4 *)(p + half);
+            *(f32x4 *)(sn + 4) = *(const f32x4 *)(p + half + 4);
+            if (lower)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sn[i] = -sn[i];
+        }
+        paged = page < A.c.pages;
+        if (!paged) flag(A.c.err, kAttnBadPage);
+        to = page * A.c.page_stride + (pos - pi * A.c.page_size) * A.c.token_stride;
+    }
+    if (A.q_norm) {
+        *(f32x4 *)wq = *(const f32x4 *)(A.q_norm + d0);
+        *(f32x4 *)(wq + 4) = *(const f32x4 *)(A.q_norm + d0 + 4);
+    }
+    if (A.k_norm) {
+        *(f32x4 *)wk = *(const f32x4 *)(A.k_norm + d0);
+        *(f32x4 *)(wk + 4) = *(const f32x4 *)(A.k_norm + d0 + 4);
+    }
+    const int other = (int)((turns ? (lower ? lane + half / 8 : lane - half / 8) : lane) * 4);
+
+    for (uint32_t x0 = xs; x0 < heads; x0 += UNROLL * xstep) {  // (the bound is over a group: its lanes stay together)
+        if (x0 != xs) load(x0);
+#pragma unroll
+        for (uint32_t u = 0; u < UNROLL; ++u) {
+            const uint32_t x = x0 + u * xstep;
+            const bool isq = x < A.q_heads, isk = !isq && x < A.q_heads + A.c.kv_heads;
+            float y[8];
+            in[u].floats(y);
+            if (isq ? A.q_norm != nullptr : isk && A.k_norm) {
+                float ss = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(y[i], y[i], ss);
+#pragma unroll
+                for (int m = LV / 2; m; m >>= 1) ss += __shfl_xor(ss, m);
+                const float r = 1.0f / __builtin_sqrtf(ss / D + A.eps);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = y[i] * r * (isq ? wq[i] : wk[i]);
+            }
+            if (A.rope && (isq || isk)) {
+                float z[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    z[i] = __int_as_float(__builtin_amdgcn_ds_bpermute(other, __float_as_int(y[i])));
+                if (turns)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(z[i], sn[i], y[i] * cs[i]);
+            }
+            if (x >= heads || !here) continue;
+            if (isq) {
+                store8<R>((uint8_t *)A.q_out + ((uint64_t)t * A.q_out_stride + x * D + d0) * kSize<R>, y);
+                continue;
+            }
+            if (!paged) continue;
+            const uint32_t h = x - A.q_heads - (isk ? 0 : A.c.kv_heads);
+            if (C == kE4M3 && (isk ? A.c.k_scale : A.c.v_scale)) {
+                const float sc = (isk ? A.c.k_scale : A.c.v_scale)[h];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = y[i] / sc;
+            }
+            store8<C>((uint8_t *)(isk ? A.c.k : A.c.v) + (to + h * A.c.head_stride + d0) * kSize<C>, y);
+        }
+    }
+}
+
+// ---- attention ------------------------------------------------------------------
+// Rows of a key head: row r of a sequence's tile list is token r / group, query
+// head h * group + r % group, so the query heads of a key head share its loads.
+//
+// Both kernels work on S^T = K Q^T and O^T = V^T P^T: the scores' result layout
+// (a lane holds one row and 4 keys in a run) is the second product's operand
+// layout once its keys are counted in that order, so weights go from one matrix
+// instruction to the next in registers; V's side of it, 4 keys of one number, is
+// what the transposing LDS read gives.
 // 8 query numbers as terms, negated where `flip` is the sign bit.
 template <uint32_t R>
 __device__ __forceinline__ void query8(const void *q, uint64_t at, uint32_t flip, bf8 (&t)[kTerms<R>]) {
@@ -283,28 +421,23 @@ __device__ __forceinline__ uint32_t lds_at(uint32_t key, uint32_t chunk) {
     return key * (D * 2) + ((chunk ^ f) << 4);
 }
 
-// Halves (bf16) of w that are not finite, as a mask.
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-    return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+// Sums over the lanes up to each one.
+template <typename T>
+__device__ __forceinline__ T wave_scan(T x) {
+    auto step = [&](auto ctrl, auto mask) {
+        x += __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl(), mask(), 0xf, false));
+    };
+    step(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // from 1 lane below in a row of 16,
+    step(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});  // 2,
+    step(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});  // 4,
+    step(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});  // 8,
+    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // rows 0 and 2 into 1 and 3,
+    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // the lower half into the upper
+    return x;
 }
-// Values that are not finite become 0, in all their terms; whether there were any.
-template <int N>
-__device__ __forceinline__ bool clean(bf8 (&v)[N]) {
-    uint32_t any = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t bad = 0;
-#pragma unroll
-        for (int t = 0; t < N; ++t) bad |= not_finite(__builtin_bit_cast(u32x4, v[t])[i]);
-#pragma unroll
-        for (int t = 0; t < N; ++t) {
-            u32x4 w = __builtin_bit_cast(u32x4, v[t]);
-            w[i] &= ~bad;
-            v[t] = __builtin_bit_cast(bf8, w);
-        }
-        any |= bad;
-    }
-    return any != 0;
+template <typename T>
+__device__ __forceinline__ T lane_of(T x, int lane) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
 }
 
 // One part of the work: keys of a row tile of a key head.
@@ -323,46 +456,36 @@ struct Item {
 template <int BM, int UNIT, bool JOIN>
 __device__ __forceinline__ bool find_item(const AttnCache &c, uint32_t group, uint32_t slots, uint32_t idx, Item &it) {
     const uint32_t lane = threadIdx.x & 63;
+    Seq s{0, 0, 0};  // of the lane's sequence; up to 64 are read once
+    auto read = [&](uint32_t b0) {
+        s = Seq{0, 0, 0};
+        if (b0 + lane < c.n) s = sequence(c, b0 + lane);
+    };
+    read(0);
     uint32_t C = 0xffffffffu;
     if (slots) {
         float total = 0;
         uint32_t tiles = 0;
-        for (uint32_t b0 = 0; b0 < c.n; b0 += 64) {
-            if (b0 + lane < c.n) {
-                const Seq s = sequence(c, b0 + lane);
-                const uint32_t t = ((uint32_t)s.nq * group + BM - 1) / BM;
-                tiles += t;
-                total += (float)t * (float)((s.len + UNIT - 1) / UNIT);
-            }
+        for (uint32_t b0 = 0;;) {
+            const uint32_t t = ((uint32_t)s.nq * group + BM - 1) / BM;
+            tiles += t;
+            total += (float)t * (float)((s.len + UNIT - 1) / UNIT);
+            if ((b0 += 64) >= c.n) break;
+            read(b0);
         }
-#pragma unroll
-        for (int m = 32; m; m >>= 1) {
-            total += __shfl_xor(total, m);
-            tiles += __shfl_xor(tiles, m);
-        }
+        total = lane_of(wave_scan(total), 63);
+        tiles = lane_of(wave_scan(tiles), 63);
         const uint32_t room = slots / c.kv_heads;
         if (tiles < room) C = max(1u, (uint32_t)__builtin_ceilf(total / (float)(room - tiles) * 1.00001f));
+        if (c.n > 64) read(0);
     }
     uint32_t base = 0, slot0 = 0;
     for (uint32_t b0 = 0; b0 < c.n; b0 += 64) {
-        Seq s{0, 0, 0};
-        uint32_t t = 0, parts = 1;
-        if (b0 + lane < c.n) {
-            s = sequence(c, b0 + lane);
-            t = ((uint32_t)s.nq * group + BM - 1) / BM;
-            const uint32_t u = (uint32_t)(s.len + UNIT - 1) / UNIT;
-            if (C != 0xffffffffu) parts = max(1u, (u + C - 1) / C);
-        }
+        if (b0) read(b0);
+        uint32_t t = ((uint32_t)s.nq * group + BM - 1) / BM, parts = 1;
+        if (C != 0xffffffffu) parts = max(1u, ((uint32_t)(s.len + UNIT - 1) / UNIT + C - 1) / C);
         const uint32_t all = t * parts * c.kv_heads, mine = JOIN ? t * c.kv_heads : all;
-        uint32_t end = mine, send = all;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const uint32_t x = __shfl_up(end, m), y = JOIN ? __shfl_up(send, m) : 0;
-            if ((int)lane >= m) {
-                end += x;
-                send += y;
-            }
-        }
+        const uint32_t end = wave_scan(mine), send = JOIN ? wave_scan(all) : 0;
         const uint64_t hit = __ballot(base + end > idx);
         if (hit) {
             const int w = __ffsll((unsigned long long)hit) - 1;
@@ -384,6 +507,70 @@ __device__ __forceinline__ bool find_item(const AttnCache &c, uint32_t group, ui
         }
         base += __builtin_amdgcn_readlane(end, 63);
         if (JOIN) slot0 += __builtin_amdgcn_readlane(send, 63);
+    }
+    return false;
+}
+
+// A share of a call's work: all tiles' units of `unit` keys, in the order sequence,
+// tile (the last first), key head, unit, dealt out evenly to `slots` workgroups
+// whatever the lengths are; a tile that several of them share is joined from their
+// sums.  slots = 0: a tile is one unit, and each workgroup takes one.
+struct Place {
+    uint32_t b, j, h, tiles, units, unit0;  // tile j of the sequence's, unit unit0 of its units
+    Seq s;
+    uint32_t start;  // number of the tile's first unit
+};
+template <int BM>
+__device__ __forceinline__ uint32_t tiles_of(const Seq &s, uint32_t group) { return ((uint32_t)s.nq * group + BM - 1) / BM; }
+__device__ __forceinline__ uint32_t units_of(const Seq &s, uint32_t unit, uint32_t slots) {
+    return slots ? max(1u, ((uint32_t)s.len + unit - 1) / unit) : 1u;
+}
+
+// Unit idx * per (JOIN: tile idx), per being the share of a workgroup.
+template <int BM, bool JOIN>
+__device__ __forceinline__ bool find_place(const AttnCache &c, uint32_t group, uint32_t slots, uint32_t unit, uint32_t idx,
+                                           uint32_t *per, Place &p) {
+    const uint32_t lane = threadIdx.x & 63;
+    Seq s{0, 0, 0};  // of the lane's sequence; up to 64 are read once
+    auto read = [&](uint32_t b0) {
+        s = Seq{0, 0, 0};
+        if (b0 + lane < c.n) s = sequence(c, b0 + lane);
+    };
+    read(0);
+    *per = 1;
+    if (slots) {
+        uint32_t total = 0;
+        for (uint32_t b0 = 0;;) {
+            total += tiles_of<BM>(s, group) * units_of(s, unit, slots);
+            if ((b0 += 64) >= c.n) break;
+            read(b0);
+        }
+        *per = max(1u, (lane_of(wave_scan(total), 63) * c.kv_heads + slots - 1) / slots);
+        if (c.n > 64) read(0);
+    }
+    const uint32_t want = JOIN ? idx : idx * *per;
+    uint32_t base = 0, start = 0;
+    for (uint32_t b0 = 0; b0 < c.n; b0 += 64) {
+        if (b0) read(b0);
+        const uint32_t t = tiles_of<BM>(s, group), u = units_of(s, unit, slots);
+        const uint32_t all = t * c.kv_heads * u, mine = JOIN ? t * c.kv_heads : all;
+        const uint32_t end = wave_scan(mine), send = JOIN ? wave_scan(all) : end;
+        const uint64_t hit = __ballot(base + end > want);
+        if (hit) {
+            const int w = __ffsll((unsigned long long)hit) - 1;
+            p.b = b0 + w;
+            p.s = Seq{lane_of(s.r0, w), lane_of(s.nq, w), lane_of(s.len, w)};
+            p.tiles = lane_of(t, w);
+            p.units = lane_of(u, w);
+            const uint32_t rel = want - (base + lane_of(end - mine, w)), tile = JOIN ? rel : rel / p.units;
+            p.unit0 = JOIN ? 0 : rel - tile * p.units;
+            p.j = tile / c.kv_heads;
+            p.h = tile - p.j * c.kv_heads;
+            p.start = start + lane_of(send - all, w) + tile * p.units;
+            return true;
+        }
+        base += lane_of(end, 63);
+        start += lane_of(send, 63);
     }
     return false;
 }
@@ -419,16 +606,6 @@ struct Runs {
             }
         }
         return at;
-    }
-    __device__ __forceinline__ void skip(const AttnCache &c, uint32_t runs) {
-        for (uint32_t i = 0; i < runs && last; ++i) {
-            --last;
-            slot += 16;
-            if (slot >= c.page_size) {
-                slot = 0;
-                ++j;
-            }
-        }
     }
 };
 
@@ -472,61 +649,45 @@ __device__ __forceinline__ f32x16 mfma32(bf8 a, bf8 b, f32x16 c) {
 
 // Where masks cut through a tile, its values that are not finite are staged as 0
 // (a masked weight of 0 would make them a NaN in rows that do not see them) and
-// added here, after the loop, to the rows that see them: products of indicators
-// count the +inf and the -inf (a NaN is both) of each number in keys from .. to.
-// Rare, so its reads are plain.  W32: results of 32 x 32 (a lane's numbers as in
-// O^T), else 16 x 16; keys in the order of the weights.
+// added here, after the loop, to the rows that see them, a key at a time: it is
+// rare.  o: a lane's numbers of O^T, of 32 x 32 products (W32) or 16 x 16.
 template <uint32_t C, int D, bool W32, typename V, int NB>
 __device__ __forceinline__ void add_not_finite(const AttnCache &c, const Item &it, int32_t from, int32_t to, int32_t sees,
                                                V (&o)[NB]) {
-    constexpr int RUN = W32 ? 16 : 32, M = W32 ? 32 : 16;
-    const uint32_t lane = threadIdx.x & 63, g = lane / M, col = lane % M;
+    constexpr int M = W32 ? 32 : 16;
+    const uint32_t d0 = (thread_id() & 63) / M * 4;
+    Runs runs;
+    runs.start(c, (uint32_t)from / 16, to);
 #pragma unroll 1
-    for (int32_t key0 = from; key0 < to; key0 += RUN) {
-        int32_t key[8];
-        bf8 vis;
+    for (int32_t run = from / 16 * 16; run < to; run += 16) {
+        const uint64_t base = runs.next(c, it, it.h * c.head_stride) + d0;
+#pragma unroll 1
+        for (int32_t key = max(run, from); key < min(run + 16, to); ++key) {
+            const uint64_t at = base + (uint64_t)(key - run) * c.token_stride;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            key[j] = key0 + (j / 4) * (RUN / 2) + (int32_t)g * 4 + j % 4;
-            vis[j] = (__bf16)(key[j] < sees ? 1.0f : 0.0f);
-        }
+            for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            bf8 up, down;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t k = (uint32_t)min(key[j], to - 1);
-                const uint32_t pg = (uint32_t)c.table[(uint64_t)it.b * c.max_pages + k / c.page_size];
-                const float x = load1<C>(c.v, (pg < c.pages ? pg : 0) * c.page_stride + it.h * c.head_stride +
-                                                  k % c.page_size * c.token_stride + i * M + col);
-                const bool in = key[j] < to;
-                up[j] = (__bf16)(in && (x != x || x == INFINITY) ? 1.0f : 0.0f);
-                down[j] = (__bf16)(in && (x != x || x == -INFINITY) ? 1.0f : 0.0f);
-            }
-            V z;
-#pragma unroll
-            for (int e = 0; e < M * M / 64; ++e) z[e] = 0.0f;
-            V n;
-            if constexpr (W32) n = mfma32(up, vis, z); else n = mfma16(up, vis, z);
-#pragma unroll
-            for (int e = 0; e < M * M / 64; ++e)
-                if (n[e] > 0.0f) o[i][e] += INFINITY;
-            if constexpr (W32) n = mfma32(down, vis, z); else n = mfma16(down, vis, z);
-#pragma unroll
-            for (int e = 0; e < M * M / 64; ++e)
-                if (n[e] > 0.0f) o[i][e] -= INFINITY;
+                for (int e = 0; e < M * M / 64; ++e) {
+                    const float x = load1<C>(c.v, at + i * M + e / 4 * 8 + e % 4);
+                    o[i][e] += key < sees && !__builtin_isfinite(x) ? x : 0.0f;
+                    if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                }
         }
     }
 }
 
 // ---- few rows on long caches: the keys split over waves and workgroups -----------
-// A workgroup takes 16 rows of one key head; its W waves take every W-th run
-// of 32 keys, each loading its keys straight into matrix operand registers and its
-// values through its own LDS tile.
+// A workgroup takes 16 rows of one key head at a time; its W waves take a W-th of
+// the keys each, KEYS at a time, loading keys straight into matrix operand
+// registers and values through their own LDS tiles.  The order of the head
+// dimension in the first product is free: lane group g holds numbers N g .. of each
+// 4 N, as one load brings them.
 template <uint32_t R, uint32_t C, int D>
 struct SplitCfg {
-    static constexpr int QT = kTerms<R>, KT = kTerms<C>, BM = 16, KEYS = 32;
+    static constexpr int QT = kTerms<R>, KT = kTerms<C>, BM = 16;
+    static constexpr int KEYS = C == kE4M3 && D <= 128 ? 64 : 32;  // about 8 KB of keys and of values in flight a wave
     static constexpr int W = KT == 3 && D == 256 ? 2 : 4, UNIT = W * KEYS;  // waves: as many as their tiles fit the LDS
+    static constexpr int OCC = D == 256 ? 1 : KT == 3 ? (D == 64 ? 2 : 1) : D == 64 ? 3 : 2;  // waves on a SIMD
     static constexpr int TILE = KEYS * D * 2;            // bytes of one plane
     static constexpr int WAVE = TILE * KT > BM * D * 4 ? TILE * KT : BM * D * 4;
     static constexpr int SLOT = BM * (D + 2);            // floats of a part's sums
@@ -537,20 +698,26 @@ __device__ __forceinline__ u32x2 read_tr(const uint8_t *lds, uint32_t at) {
 }
 
 template <uint32_t R, uint32_t C, int D>
-__global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W)) void k_attn_split(AttnArgs A, uint32_t slots) {
+__global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OCC)) void k_attn_split(AttnArgs A, uint32_t slots,
+                                                                                                 uint32_t unit) {
     using G = SplitCfg<R, C, D>;
-    constexpr int QT = G::QT, KT = G::KT, W = G::W, NS = D / 32, NB = D / 16, NV = 32 * D / 8 / 64;
+    constexpr int QT = G::QT, KT = G::KT, W = G::W, NS = D / 32, NB = D / 16, KEYS = G::KEYS, NR = KEYS / 16;
+    constexpr int PN = Piece<C>::N, SUB = PN / 8, NK = NS / SUB, NV = KEYS * D / PN / 64;
     __shared__ __align__(16) uint8_t sh[W * G::WAVE];
     __shared__ float sh_m[W][16], sh_l[W][16];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t g = lane >> 4, col = lane & 15;
-    Item it;
-    if (!find_item<G::BM, G::UNIT, false>(A.c, A.group, slots, blockIdx.x, it)) return;
-    int32_t end;
-    uint32_t per, parts;
-    tile_keys<G::BM, G::UNIT>(it, A.group, &end, &per, &parts);
-    if (it.part >= parts) return;
-    const int32_t first = (int32_t)(it.part * per * G::UNIT), stop = min(end, first + (int32_t)(per * G::UNIT));
+    Place pl;
+    uint32_t left;
+    if (!find_place<G::BM, false>(A.c, A.group, slots, unit, blockIdx.x, &left, pl)) return;
+    // tile after tile until the share is used up
+    for (;; __syncthreads()) {
+    const Item it{pl.b, pl.tiles - 1 - pl.j, pl.h, 0, 0, 0, pl.s.r0, pl.s.nq, pl.s.len};
+    const uint32_t take = min(left, pl.units - pl.unit0);
+    const bool whole = take == pl.units;
+    const uint32_t last = min((it.rt + 1) * 16, (uint32_t)it.nq * A.group) - 1;
+    const int32_t end = max(0, it.len - it.nq + (int32_t)(last / A.group) + 1);
+    const int32_t first = slots ? (int32_t)(pl.unit0 * unit) : 0, stop = slots ? min(end, first + (int32_t)(take * unit)) : end;
 
     const uint32_t r = it.rt * 16 + col, rows = (uint32_t)it.nq * A.group;
     const bool valid = r < rows;
@@ -564,7 +731,8 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W)) void k_attn_split(Attn
 
     bf8 q[NS][QT];
 #pragma unroll
-    for (int s = 0; s < NS; ++s) query8<R>(A.q, row * A.q_stride + (uint64_t)x * D + s * 32 + g * 8, flip, q[s]);
+    for (int s = 0; s < NS; ++s)
+        query8<R>(A.q, row * A.q_stride + (uint64_t)x * D + s / SUB * 4 * PN + g * PN + s % SUB * 8, flip, q[s]);
 
     f32x4 o[NB];
 #pragma unroll
@@ -574,70 +742,87 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W)) void k_attn_split(Attn
 
     const uint64_t head = it.h * A.c.head_stride;
     Runs runs;
-    runs.start(A.c, (uint32_t)(first / 16) + wave * 2, end);
-    Eight<C> kr[2][NS], vr[NV];
-    const uint32_t ts = (uint32_t)A.c.token_stride, klane = (col * ts + g * 8) * kSize<C>;
-    auto load = [&] {
-        const uint8_t *kb[2], *vb[2];
+    const int32_t share = (max(0, stop - first) + W * KEYS - 1) / (W * KEYS) * KEYS;  // keys of a wave
+    const int32_t wfirst = first + (int32_t)wave * share, wstop = min(stop, wfirst + share);
+    runs.start(A.c, (uint32_t)wfirst / 16, end);
+    Piece<C> kr[NR][NK], vr[NV];
+    // addresses: a scalar base for a run of keys or a load of values, and one offset a lane for each kind
+    const uint32_t ts = (uint32_t)A.c.token_stride * kSize<C>, klane = col * ts + g * PN * kSize<C>;
+    const uint32_t vlane = lane / (D / PN) * ts + lane % (D / PN) * PN * kSize<C>;
+    uint64_t base[NR];
+    auto load_keys = [&] {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const uint64_t at = runs.next(A.c, it, head) * kSize<C>;
-            kb[n] = (const uint8_t *)A.c.k + at;
-            vb[n] = (const uint8_t *)A.c.v + at;
-        }
-        runs.skip(A.c, 2 * (W - 1));
+        for (int n = 0; n < NR; ++n) {
+            base[n] = runs.next(A.c, it, head) * kSize<C>;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-                kr[n][s].load(kb[n] + (klane + s * 32 * kSize<C>));
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t id = i * 64 + lane, key = id / (D / 8), ch = id % (D / 8);
-            vr[i].load(vb[i * 64 / (D / 8) / 16] + ((key & 15) * ts + ch * 8) * kSize<C>);
+            for (int s = 0; s < NK; ++s) kr[n][s].load((const uint8_t *)A.c.k + base[n] + klane + s * 4 * PN * kSize<C>);
         }
     };
-    int32_t key0 = first + (int32_t)wave * 32, bad_at = -1;
-    if (key0 < stop) load();
-    for (; key0 < stop; key0 += G::UNIT) {
-        f32x4 sc[2];
+    auto load_values = [&] {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int i = 0; i < NV; ++i) {
+            constexpr int KL = 64 / (D / PN);  // keys a load
+            vr[i].load((const uint8_t *)A.c.v + base[i * KL / 16] + i * KL % 16 * ts + vlane);
+        }
+    };
+    int32_t bad_at = -1;
+    if (wfirst < wstop) {
+        load_keys();
+        load_values();
+    }
+    for (int32_t key0 = wfirst; key0 < wstop; key0 += KEYS) {
+        f32x4 sc[NR];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
             sc[n] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 bf8 k[KT];
-                kr[n][s].terms(k);
+                kr[n][s / SUB].terms(s % SUB, k);
                 sc[n] = product<KT, QT>(k, q[s], sc[n], mfma16);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if (key0 + KEYS < wstop) load_keys();
         // values into the wave's tile; what is behind the sequence's end counts as 0
-        const bool tail = key0 + 32 > it.len, masked = key0 + 32 > sees_min;
-        bool bad = false;
+        const bool masked = key0 + KEYS > sees_min;
+        if (masked) {
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (key0 + (int32_t)((i * 64 + lane) / (D / PN)) >= it.len) vr[i].zero();
+                bad |= vr[i].clean();
+            }
+            if (bad_at < 0 && __any(bad)) bad_at = key0;
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const uint32_t id = i * 64 + lane, key = id / (D / 8), ch = id % (D / 8);
-            if (tail && key0 + (int32_t)key >= it.len) vr[i].zero();
-            bf8 v[KT];
-            vr[i].terms(v);
-            if (masked) bad |= clean(v);
+            const uint32_t id = i * 64 + lane, key = id / (D / PN), ch = id % (D / PN);
 #pragma unroll
-            for (int t = 0; t < KT; ++t) *(bf8 *)(lds + t * G::TILE + lds_at<D>(key, ch)) = v[t];
+            for (int u = 0; u < SUB; ++u) {
+                bf8 v[KT];
+                vr[i].terms(u, v);
+#pragma unroll
+                for (int t = 0; t < KT; ++t) *(bf8 *)(lds + t * G::TILE + lds_at<D>(key, ch * SUB + u)) = v[t];
+            }
         }
-        if (bad_at < 0 && __any(bad)) bad_at = key0;
-        if (key0 + G::UNIT < stop) load();
+        if (key0 + KEYS < wstop) load_values();
+        __builtin_amdgcn_sched_barrier(0);
 
         float cc = c2;
         if (masked) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NR; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     sc[n][i] = key0 + n * 16 + (int32_t)g * 4 + i < sees ? sc[n][i] * c2 : -INFINITY;
             cc = 1.0f;
         }
-        float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                         fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+        float mx = sc[0][0];
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[n][i]);
         mx = across32(across16(mx)) * cc;
         if (__any(mx > st.m + 8.0f)) {
             const float mn = fmaxf(st.m, mx), f = exp2_hw(st.m - finite_max(mn));
@@ -647,52 +832,52 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W)) void k_attn_split(Attn
             st.m = mn;
         }
         const float mu = finite_max(st.m);
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            p[i] = exp2_hw(__builtin_fmaf(sc[i / 4][i % 4], cc, -mu));
-            st.l += p[i];
-        }
-        bf8 pt[QT];
-        split8<QT>(p, pt);
-
         const uint32_t tk = g * 4 + (col >> 2), tc = (col & 3) >> 1, tb = (col & 1) * 8;
-        auto values = [&](int i, bf8 (&v)[KT]) {
 #pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const uint32_t at = t * G::TILE + lds_at<D>(tk, i * 2 + tc) + tb;
-                const u32x2 a = read_tr(lds, at), b = read_tr(lds, at + 16 * D * 2);
-                v[t] = __builtin_bit_cast(bf8, u32x4{a[0], a[1], b[0], b[1]});
+        for (int n = 0; n < NR; n += 2) {
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                p[i] = exp2_hw(__builtin_fmaf(sc[n + i / 4][i % 4], cc, -mu));
+                st.l += p[i];
             }
-        };
+            bf8 pt[QT];
+            split8<QT>(p, pt);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            bf8 v[KT];
-            values(i, v);
-            o[i] = product<KT, QT>(v, pt, o[i], mfma16);
+            for (int i = 0; i < NB; ++i) {
+                bf8 v[KT];
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    const uint32_t at = t * G::TILE + lds_at<D>(tk, i * 2 + tc) + tb + n * 16 * D * 2;
+                    const u32x2 a = read_tr(lds, at), b = read_tr(lds, at + 16 * D * 2);
+                    v[t] = __builtin_bit_cast(bf8, u32x4{a[0], a[1], b[0], b[1]});
+                }
+                o[i] = product<KT, QT>(v, pt, o[i], mfma16);
+            }
         }
         __builtin_amdgcn_wave_barrier();
     }
-    if (bad_at >= 0)
-        for (int32_t k = bad_at; k < stop; k += G::UNIT)
-            add_not_finite<C, D, false>(A.c, it, k, min(k + 32, min(stop, it.len)), sees, o);
+    if (bad_at >= 0) add_not_finite<C, D, false>(A.c, it, bad_at, min(wstop, it.len), sees, o);
 
     // the waves' sums
+    const uint32_t tid = thread_id(), ecol = tid & 15, eg = tid >> 4 & 3;
     st.l += __shfl_xor(st.l, 16);
     st.l += __shfl_xor(st.l, 32);
-    if (lane < 16) {
-        sh_m[wave][col] = st.m;
-        sh_l[wave][col] = st.l;
+    if (eg == 0) {
+        sh_m[wave][ecol] = st.m;
+        sh_l[wave][ecol] = st.l;
     }
     float *const mine = (float *)lds;
 #pragma unroll
-    for (int i = 0; i < NB; ++i) *(f32x4 *)(mine + col * D + ((i * 16 + g * 4) ^ ((col & 7) << 2))) = o[i];
+    for (int i = 0; i < NB; ++i) *(f32x4 *)(mine + ecol * D + ((i * 16 + eg * 4) ^ ((ecol & 7) << 2))) = o[i];
     __syncthreads();
-    float *const part = (float *)A.work + (uint64_t)it.slot * G::SLOT;
+    // a workgroup's share starts with at most one tile's end and ends with at most one tile's start
+    float *const part = (float *)A.work + (2 * (uint64_t)blockIdx.x + (pl.unit0 == 0)) * G::SLOT;
     const float vs = C == kE4M3 && A.c.v_scale ? A.c.v_scale[it.h] : 1.0f;
 #pragma unroll
     for (int e = 0; e < 16 * D / 4 / (64 * W); ++e) {
-        const uint32_t id = e * 64 * W + threadIdx.x, rr = id / (D / 4), d = id % (D / 4) * 4;
+        const uint32_t id = e * 64 * W + tid, rr = id / (D / 4), d = id % (D / 4) * 4;
         const uint32_t tr = it.rt * 16 + rr;
         if (tr >= rows) continue;
         float m = -INFINITY;
@@ -709,7 +894,7 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W)) void k_attn_split(Attn
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = __builtin_fmaf(z[i], f, y[i]);
         }
-        if (parts > 1) {
+        if (!whole) {
             *(f32x4 *)(part + rr * D + d) = y;
             if (d == 0) {
                 part[16 * D + rr] = m;
@@ -721,43 +906,101 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W)) void k_attn_split(Attn
                       it.len - it.nq + (int32_t)t + 1 > 0 ? vs / l : 0.0f);
         }
     }
+    left -= take;
+    if (!left) return;
+    pl.unit0 = 0;
+    if (++pl.h == A.c.kv_heads) {
+        pl.h = 0;
+        if (++pl.j == pl.tiles) {
+            pl.j = 0;
+            do {
+                if (++pl.b == A.c.n) return;
+                const Seq s = sequence(A.c, pl.b);
+                pl.s = Seq{__builtin_amdgcn_readfirstlane(s.r0), __builtin_amdgcn_readfirstlane(s.nq),
+                           __builtin_amdgcn_readfirstlane(s.len)};
+                pl.tiles = tiles_of<G::BM>(pl.s, A.group);
+            } while (!pl.tiles);
+            pl.units = units_of(pl.s, unit, slots);
+        }
+    }
+    }
 }
 
-// Joins the parts of a tile of BM rows: a workgroup per 16 rows.
-template <uint32_t R, uint32_t C, int D, int BM, int UNIT>
-__global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots) {
+// Joins the parts of a tile.  LD lanes read LD * 4 numbers of a part's row; a
+// workgroup takes ROWS rows of them, NG groups of lanes sharing a row's parts.
+// UNIT > 0: of the prompt kernel's parts, else of shares of units of `unit` keys.
+template <uint32_t R, uint32_t C, int D, int BM, int UNIT, int LD, int ROWS>
+__global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots, uint32_t unit) {
+    constexpr uint32_t NG = 256 / LD / ROWS, BLOCKS = BM / ROWS, SLOT = BM * (D + 2);
     Item it;
-    const uint32_t sub = blockIdx.x % (BM / 16);
-    if (!find_item<BM, UNIT, true>(A.c, A.group, slots, blockIdx.x / (BM / 16), it)) return;
-    int32_t end;
-    uint32_t per, parts;
-    tile_keys<BM, UNIT>(it, A.group, &end, &per, &parts);
-    if (parts == 1) return;
-    const float vs = C == kE4M3 && A.c.v_scale ? A.c.v_scale[it.h] : 1.0f;
-    const float *const first = (const float *)A.work + (uint64_t)it.slot * (BM * (D + 2));
-    const uint64_t step = (uint64_t)A.c.kv_heads * (BM * (D + 2));
-    const uint32_t rows = (uint32_t)it.nq * A.group;
-#pragma unroll
-    for (int e = 0; e < 16 * D / 4 / 256; ++e) {
-        const uint32_t id = e * 256 + threadIdx.x, rr = sub * 16 + id / (D / 4), d = id % (D / 4) * 4;
-        const uint32_t tr = it.rt * BM + rr;
-        if (tr >= rows) continue;
-        float m = -INFINITY, l = 0;
-        for (uint32_t p = 0; p < parts; ++p) m = fmaxf(m, first[p * step + BM * D + rr]);
-        const float mf = finite_max(m);
-        f32x4 y{0, 0, 0, 0};
-        for (uint32_t p = 0; p < parts; ++p) {
-            const float *const s = first + p * step;
-            const float f = exp2_hw(s[BM * D + rr] - mf);
-            const f32x4 z = *(const f32x4 *)(s + rr * D + d);
-            l = __builtin_fmaf(s[BM * D + BM + rr], f, l);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = __builtin_fmaf(z[i], f, y[i]);
-        }
-        const uint32_t t = tr / A.group;
-        write4<R>(A, (uint64_t)it.r0 + t, it.h * A.group + tr - t * A.group, D, d, y,
-                  it.len - it.nq + (int32_t)t + 1 > 0 ? vs / l : 0.0f);
+    const uint32_t rb = blockIdx.x % BLOCKS * ROWS, rr = rb + threadIdx.x / (LD * NG);
+    uint32_t parts;
+    uint64_t slot0, next;  // the first part's sums, and from the second's to the next
+    if constexpr (UNIT > 0) {
+        if (!find_item<BM, UNIT, true>(A.c, A.group, slots, blockIdx.x / BLOCKS, it)) return;
+        int32_t end;
+        uint32_t per;
+        tile_keys<BM, UNIT>(it, A.group, &end, &per, &parts);
+        slot0 = it.slot;
+        next = A.c.kv_heads;
+    } else {
+        Place p;
+        uint32_t per;
+        if (!find_place<BM, true>(A.c, A.group, slots, unit, blockIdx.x / BLOCKS, &per, p)) return;
+        const uint32_t w = p.start / per;
+        parts = (p.start + p.units - 1) / per - w + 1;
+        slot0 = 2 * (uint64_t)w;
+        next = 2;
+        it = Item{p.b, p.tiles - 1 - p.j, p.h, 0, 0, 0, p.s.r0, p.s.nq, p.s.len};
     }
+    const uint32_t tr = it.rt * BM + rr;
+    if (parts == 1 || it.rt * BM + rb >= (uint32_t)it.nq * A.group) return;
+    const float *const first = (const float *)A.work + slot0 * SLOT;
+    const uint64_t step = next * SLOT;
+    const uint32_t pg = threadIdx.x / LD % NG, dl = threadIdx.x % LD, d = (blockIdx.y * LD + dl) * 4;
+    // a group keeps its own running maximum; the groups are joined like the parts
+    float m = -INFINITY, l = 0;
+    f32x4 y{0, 0, 0, 0};
+    for (uint32_t p = pg; p < parts; p += NG) {
+        const float *const s = first + p * step + (UNIT == 0 && p == 0 ? SLOT : 0);
+        const float pm = s[BM * D + rr], pl = s[BM * D + BM + rr];
+        const f32x4 z = *(const f32x4 *)(s + rr * D + d);
+        const float mn = fmaxf(m, pm), f0 = exp2_hw(m - finite_max(mn)), f1 = exp2_hw(pm - finite_max(mn));
+        m = mn;
+        l = __builtin_fmaf(pl, f1, l * f0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = __builtin_fmaf(z[i], f1, y[i] * f0);
+    }
+    if constexpr (NG > 1) {
+        __shared__ float sh_m[ROWS][NG], sh_l[ROWS][NG];
+        __shared__ f32x4 sh_y[ROWS][NG][LD];
+        const uint32_t w = threadIdx.x / (LD * NG);
+        if (dl == 0) {
+            sh_m[w][pg] = m;
+            sh_l[w][pg] = l;
+        }
+        sh_y[w][pg][dl] = y;
+        __syncthreads();
+        if (pg) return;
+        m = sh_m[w][0];
+#pragma unroll
+        for (uint32_t i = 1; i < NG; ++i) m = fmaxf(m, sh_m[w][i]);
+        const float mf = finite_max(m);
+        l = 0;
+        y = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t g = 0; g < NG; ++g) {
+            const float f = exp2_hw(sh_m[w][g] - mf);
+            l = __builtin_fmaf(sh_l[w][g], f, l);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = __builtin_fmaf(sh_y[w][g][dl][i], f, y[i]);
+        }
+    }
+    if (tr >= (uint32_t)it.nq * A.group) return;
+    const uint32_t t = tr / A.group;
+    const float vs = C == kE4M3 && A.c.v_scale ? A.c.v_scale[it.h] : 1.0f;
+    write4<R>(A, (uint64_t)it.r0 + t, it.h * A.group + tr - t * A.group, D, d, y,
+              it.len - it.nq + (int32_t)t + 1 > 0 ? vs / l : 0.0f);
 }
 
 // ---- prompts ---------------------------------------------------------------------
@@ -776,7 +1019,8 @@ struct TileCfg {
 template <uint32_t R, uint32_t C, int D>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A, uint32_t slots) {
     using G = TileCfg<R, C, D>;
-    constexpr int QT = G::QT, KT = G::KT, BK = G::BK, NS = D / 16, NB = D / 32, NN = BK / 32, NL = BK * D / 8 / 256;
+    constexpr int QT = G::QT, KT = G::KT, BK = G::BK, NS = D / 16, NB = D / 32, NN = BK / 32;
+    constexpr int PN = Piece<C>::N, SUB = PN / 8, NL = BK * D / PN / 256;
     __shared__ __align__(16) uint8_t sh[G::BUF * 2 * G::HALF];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t g = lane >> 5, col = lane & 31;
@@ -814,11 +1058,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
     const uint64_t head = it.h * A.c.head_stride;
     Runs runs;
     runs.start(A.c, (uint32_t)(first / 16), end);
-    Eight<C> kr[NL], vr[NL];
-    // a thread's pieces: 8 numbers of key id / (D / 8), so a wave's are of one run
-    const uint32_t ch = threadIdx.x % (D / 8), tkey = threadIdx.x / (D / 8);
-    const uint32_t voff = ((tkey & 15) * (uint32_t)A.c.token_stride + ch * 8) * kSize<C>;
-    constexpr int STEP = 256 / (D / 8);  // keys from one piece of a thread to its next
+    Piece<C> kr[NL], vr[NL];
+    // thread t's pieces are of keys t / (D / PN) + STEP i, so a wave's are of one run
+    const uint32_t ch = threadIdx.x % (D / PN), tkey = threadIdx.x / (D / PN);
+    const uint32_t voff = ((tkey & 15) * (uint32_t)A.c.token_stride + ch * PN) * kSize<C>;
+    constexpr int STEP = 256 / (D / PN);  // keys from one piece of a thread to its next
     const uint32_t vnext = STEP < 16 ? STEP * (uint32_t)A.c.token_stride * kSize<C> : 0;
     auto load = [&] {
         uint64_t base[BK / 16];
@@ -830,7 +1074,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
             constexpr int PER = STEP >= 16 ? STEP / 16 : 1;
             uint64_t at = base[STEP >= 16 ? i * PER : i * STEP / 16];
             if constexpr (PER > 1) {
-                const uint32_t run = wave * 64 / (D / 8) / 16;
+                const uint32_t run = wave * 64 / (D / PN) / 16;
 #pragma unroll
                 for (int n = 1; n < PER; ++n) at = run == n ? base[i * PER + n] : at;
             }
@@ -843,19 +1087,26 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
     const int32_t cut = min(max(it.len - it.nq + (int32_t)(it.rt * G::BM / A.group) + 1, 0), end);
     bool bad = false;
     auto store = [&](int32_t key0, uint8_t *to) {
-        const bool tail = key0 + BK > it.len, masked = key0 + BK > cut;
+        if (key0 + BK > cut) {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                if (key0 + (int32_t)(i * STEP + tkey) >= it.len) vr[i].zero();
+                bad |= vr[i].clean();
+            }
+        }
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const uint32_t key = i * STEP + tkey;
-            if (tail && key0 + (int32_t)key >= it.len) vr[i].zero();
-            bf8 k[KT], v[KT];
-            kr[i].terms(k);
-            vr[i].terms(v);
-            if (masked) bad |= clean(v);
 #pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                *(bf8 *)(to + t * G::PLANE + lds_at<D>(tkey, ch) + i * STEP * D * 2) = k[t];
-                *(bf8 *)(to + G::HALF + t * G::PLANE + lds_at<D>(tkey, ch) + i * STEP * D * 2) = v[t];
+            for (int u = 0; u < SUB; ++u) {
+                bf8 k[KT], v[KT];
+                kr[i].terms(u, k);
+                vr[i].terms(u, v);
+                const uint32_t at = lds_at<D>(tkey, ch * SUB + u) + i * STEP * D * 2;
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    *(bf8 *)(to + t * G::PLANE + at) = k[t];
+                    *(bf8 *)(to + G::HALF + t * G::PLANE + at) = v[t];
+                }
             }
         }
     };
@@ -987,53 +1238,76 @@ void pick(uint32_t row_t, uint32_t cache_t, uint32_t dim, F &&f) {
 
 }  // namespace
 
+// Rows from which a workgroup takes eight.
+constexpr uint32_t kAppendBlockRows = 2048;
+
 void launch_append(const AppendArgs &A, uint32_t row_t, uint32_t dim, hipStream_t st) {
-    const uint64_t items = (uint64_t)A.c.rows * (A.q_heads + 2 * A.c.kv_heads);
     pick(row_t, A.c.dtype, dim, [&](auto r, auto c, auto d) {
-        k_append<r(), c(), d()><<<(uint32_t)((items + 3) / 4), 256, 0, st>>>(A);
+        constexpr uint32_t groups = 256 / (d() / 8);
+        if (A.c.rows >= kAppendBlockRows)
+            k_append<r(), c(), d(), 8><<<(A.c.rows + 7) / 8, 256, 0, st>>>(A);
+        else
+            k_append<r(), c(), d(), 1><<<dim3(A.c.rows, (A.q_heads + 2 * A.c.kv_heads + groups - 1) / groups), 256, 0, st>>>(A);
     });
 }
 
 namespace {
 
-// Workgroups that share a call's work when its row tiles are fewer: two on a CU.
-constexpr uint32_t kSplitSlots = 512, kTileSlots = 512;
-
 struct Plan {
     bool tile;              // the prompt kernel
     uint32_t tiles, slots;  // row tiles x key heads at most; workgroups that share them (0: one for each tile)
+    uint32_t unit;          // keys that go to one of them together
 };
 
-Plan plan(const AttnArgs &A) {
+Plan plan(const AttnArgs &A, uint32_t dim) {
     Plan p;
     const uint64_t rows = (uint64_t)A.c.rows * A.group;
     p.tile = A.c.row0 && rows > 64ull * A.c.n;
-    const uint32_t bm = p.tile ? 128 : 16, want = p.tile ? kTileSlots : kSplitSlots;
+    const uint32_t bm = p.tile ? 128 : 16;
     // a sequence's last tile may be in part empty
     p.tiles = (uint32_t)std::min<uint64_t>(rows / bm + A.c.n, rows) * A.c.kv_heads;
-    p.slots = p.tiles < want ? want : 0;
+    if (p.tile) {
+        p.slots = p.tiles < 512 ? 512 : 0;  // two workgroups on a CU
+        p.unit = 0;
+        return p;
+    }
+    // as many workgroups as are on the chip at once, or tiles where those are more: shorter shares, which
+    // the chip takes in turn; many tiles need no sharing
+    const bool f32 = A.c.dtype == kF32;
+    const uint32_t chip = dim == 256 || (f32 && dim == 128) ? 256 : 512;
+    p.slots = p.tiles < 2048 ? std::max(chip, p.tiles) : 0;
+    p.unit = f32 && dim == 256 ? 64 : A.c.dtype == kE4M3 && dim <= 128 ? 256 : 128;  // SplitCfg::UNIT
+    while ((uint64_t)p.tiles * ((uint64_t)A.c.max_pages * A.c.page_size / p.unit + 2) > 0x7fffffffull) p.unit *= 2;
     return p;
 }
 
 }  // namespace
 
 uint64_t attn_work_bytes(const AttnArgs &A, uint32_t dim) {
-    const Plan p = plan(A);
-    return std::max<uint64_t>(16, (uint64_t)p.slots * (p.tile ? 128 : 16) * (dim + 2) * 4);
+    const Plan p = plan(A, dim);
+    return std::max<uint64_t>(16, (uint64_t)p.slots * (p.tile ? 128 : 2 * 16) * (dim + 2) * 4);
 }
 
 void launch_attn(const AttnArgs &A, uint32_t row_t, uint32_t dim, hipStream_t st) {
-    const Plan p = plan(A);
-    const uint32_t grid = std::max(p.tiles, p.slots);
+    const Plan p = plan(A, dim);
+    const uint32_t grid = p.tile ? std::max(p.tiles, p.slots) : p.slots ? p.slots : p.tiles;
+    // with many parts a tile, a workgroup joins 32 numbers of a row, else as many rows as its lanes hold
+    auto join = [&](auto r, auto c, auto d, auto bm, auto unit) {
+        constexpr int all = 1024 / d() < bm() ? 1024 / d() : bm();
+        if (p.slots > 16 * p.tiles)
+            k_attn_join<r(), c(), d(), bm(), unit(), 8, 1><<<dim3(p.tiles * bm(), d() / 32), 256, 0, st>>>(A, p.slots, p.unit);
+        else if (p.slots)
+            k_attn_join<r(), c(), d(), bm(), unit(), d() / 4, all><<<p.tiles * (bm() / all), 256, 0, st>>>(A, p.slots, p.unit);
+    };
     pick(row_t, A.c.dtype, dim, [&](auto r, auto c, auto d) {
         if (p.tile) {
             using G = TileCfg<r(), c(), d()>;
             k_attn_tile<r(), c(), d()><<<grid, 256, 0, st>>>(A, p.slots);
-            if (p.slots) k_attn_join<r(), c(), d(), G::BM, G::BK><<<p.tiles * (G::BM / 16), 256, 0, st>>>(A, p.slots);
+            join(r, c, d, std::integral_constant<int, G::BM>{}, std::integral_constant<int, G::BK>{});
         } else {
             using G = SplitCfg<r(), c(), d()>;
-            k_attn_split<r(), c(), d()><<<grid, 64 * G::W, 0, st>>>(A, p.slots);
-            if (p.slots) k_attn_join<r(), c(), d(), G::BM, G::UNIT><<<p.tiles, 256, 0, st>>>(A, p.slots);
+            k_attn_split<r(), c(), d()><<<grid, 64 * G::W, 0, st>>>(A, p.slots, p.unit);
+            join(r, c, d, std::integral_constant<int, G::BM>{}, std::integral_constant<int, 0>{});
         }
     });
 }
