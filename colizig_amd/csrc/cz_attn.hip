@@ -118,6 +118,10 @@ struct Eight<kF32> {
         a = *(const u32x4 *)p;
         b = *(const u32x4 *)(p + 16);
     }
+    __device__ __forceinline__ void load_once(const uint8_t *p) {
+        a = __builtin_nontemporal_load((const u32x4 *)p);
+        b = __builtin_nontemporal_load((const u32x4 *)(p + 16));
+    }
     __device__ __forceinline__ void zero() { a = b = u32x4{0, 0, 0, 0}; }
     __device__ __forceinline__ void floats(float (&x)[8]) const {
 #pragma unroll
@@ -136,6 +140,7 @@ template <>
 struct Eight<kBF16> {
     u32x4 a;
     __device__ __forceinline__ void load(const uint8_t *p) { a = *(const u32x4 *)p; }
+    __device__ __forceinline__ void load_once(const uint8_t *p) { a = __builtin_nontemporal_load((const u32x4 *)p); }
     __device__ __forceinline__ void zero() { a = u32x4{0, 0, 0, 0}; }
     __device__ __forceinline__ void floats(float (&x)[8]) const {
 #pragma unroll
@@ -180,11 +185,14 @@ __device__ __forceinline__ bool clean(uint32_t &w) {
 }
 
 // What a lane loads at a time: 8 numbers, of an E4M3 cache 16 so that it is 16 bytes.
+// load_once: of data that nobody reads again (keeps the caches for what is; 533 MB of
+// BF16 keys and values of one token go from 101 to 92 us with it).
 template <uint32_t T>
 struct Piece {
     static constexpr int N = 8;
     Eight<T> e;
     __device__ __forceinline__ void load(const uint8_t *p) { e.load(p); }
+    __device__ __forceinline__ void load_once(const uint8_t *p) { e.load_once(p); }
     __device__ __forceinline__ void zero() { e.zero(); }
     __device__ __forceinline__ bool clean() {
         bool any = false;
@@ -208,6 +216,7 @@ struct Piece<kE4M3> {
     static constexpr int N = 16;
     u32x4 a;
     __device__ __forceinline__ void load(const uint8_t *p) { a = *(const u32x4 *)p; }
+    __device__ __forceinline__ void load_once(const uint8_t *p) { a = __builtin_nontemporal_load((const u32x4 *)p); }
     __device__ __forceinline__ void zero() { a = u32x4{0, 0, 0, 0}; }
     __device__ __forceinline__ bool clean() {
         bool any = false;
@@ -412,12 +421,13 @@ __device__ __forceinline__ V product(const bf8 (&a)[NA], const bf8 (&b)[NB], V c
 }
 
 // Where 16-byte piece `chunk` of bf16 row `key` sits in an LDS tile of D numbers a
-// row: the pieces of a row are permuted by the key so that 8 lanes' pieces of K (8
-// keys), and the 4 keys x 32 bytes that 16 lanes read of V, fall on different
-// banks.  Keys 8 apart are permuted alike: one address serves both.
+// row: the pieces of a row are permuted by the key, so that what the LDS serves at
+// once falls on different banks: 8 keys at one piece (a read of K), and 4 keys at 4
+// pieces, or 8 at 2 (the transposing reads of V).  Keys 8 apart are permuted alike:
+// one address serves both.
 template <int D>
 __device__ __forceinline__ uint32_t lds_at(uint32_t key, uint32_t chunk) {
-    const uint32_t f = ((key & 7) << 1) & (D / 8 - 1);
+    const uint32_t f = D == 64 ? (key & 2) << 1 | (key & 4) >> 1 : (key & 3) << 2 | (key & 4) >> 1;
     return key * (D * 2) + ((chunk ^ f) << 4);
 }
 
@@ -710,20 +720,88 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
     Place pl;
     uint32_t left;
     if (!find_place<G::BM, false>(A.c, A.group, slots, unit, blockIdx.x, &left, pl)) return;
-    // tile after tile until the share is used up
-    for (;; __syncthreads()) {
-    const Item it{pl.b, pl.tiles - 1 - pl.j, pl.h, 0, 0, 0, pl.s.r0, pl.s.nq, pl.s.len};
-    const uint32_t take = min(left, pl.units - pl.unit0);
-    const bool whole = take == pl.units;
-    const uint32_t last = min((it.rt + 1) * 16, (uint32_t)it.nq * A.group) - 1;
-    const int32_t end = max(0, it.len - it.nq + (int32_t)(last / A.group) + 1);
-    const int32_t first = slots ? (int32_t)(pl.unit0 * unit) : 0, stop = slots ? min(end, first + (int32_t)(take * unit)) : end;
 
+    // A tile of the share: its rows, and the wave's keys.
+    struct Segment {
+        Item it;
+        uint32_t take;
+        bool whole, opens;          // all of the tile's units; its first ones
+        int32_t end, first, stop;   // keys that its last row sees; the wave's
+    };
+    auto segment = [&] {
+        Segment sg;
+        sg.it = Item{pl.b, pl.tiles - 1 - pl.j, pl.h, 0, 0, 0, pl.s.r0, pl.s.nq, pl.s.len};
+        sg.take = min(left, pl.units - pl.unit0);
+        sg.whole = sg.take == pl.units;
+        sg.opens = pl.unit0 == 0;
+        const uint32_t last = min((sg.it.rt + 1) * 16, (uint32_t)sg.it.nq * A.group) - 1;
+        sg.end = max(0, sg.it.len - sg.it.nq + (int32_t)(last / A.group) + 1);
+        const int32_t f = slots ? (int32_t)(pl.unit0 * unit) : 0;
+        const int32_t st = slots ? min(sg.end, f + (int32_t)(sg.take * unit)) : sg.end;
+        const int32_t share = (max(0, st - f) + W * KEYS - 1) / (W * KEYS) * KEYS;
+        sg.first = f + (int32_t)wave * share;
+        sg.stop = min(st, sg.first + share);
+        return sg;
+    };
+    // the tile after it; the next sequence has been read ahead
+    Seq ahead = sequence(A.c, min(pl.b + 1, A.c.n - 1));
+    auto advance = [&](uint32_t took) {
+        left -= took;
+        if (!left) return false;
+        pl.unit0 = 0;
+        if (++pl.h < A.c.kv_heads) return true;
+        pl.h = 0;
+        if (++pl.j < pl.tiles) return true;
+        pl.j = 0;
+        do {
+            if (++pl.b == A.c.n) return false;
+            pl.s = Seq{__builtin_amdgcn_readfirstlane(ahead.r0), __builtin_amdgcn_readfirstlane(ahead.nq),
+                       __builtin_amdgcn_readfirstlane(ahead.len)};
+            pl.tiles = tiles_of<G::BM>(pl.s, A.group);
+            ahead = sequence(A.c, min(pl.b + 1, A.c.n - 1));
+        } while (!pl.tiles);
+        pl.units = units_of(pl.s, unit, slots);
+        return true;
+    };
+
+    Runs runs;
+    Piece<C> kr[NR][NK], vr[NV];
+    // addresses: a scalar base for a run of keys or a load of values, and one offset a lane for each kind
+    const uint32_t ts = (uint32_t)A.c.token_stride * kSize<C>, klane = col * ts + g * PN * kSize<C>;
+    const uint32_t vlane = lane / (D / PN) * ts + lane % (D / PN) * PN * kSize<C>;
+    uint64_t base[NR];
+    auto load_keys = [&](const Item &it) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            base[n] = runs.next(A.c, it, it.h * A.c.head_stride) * kSize<C>;
+#pragma unroll
+            for (int s = 0; s < NK; ++s) kr[n][s].load_once((const uint8_t *)A.c.k + base[n] + klane + s * 4 * PN * kSize<C>);
+        }
+    };
+    auto load_values = [&] {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            constexpr int KL = 64 / (D / PN);  // keys a load
+            vr[i].load_once((const uint8_t *)A.c.v + base[i * KL / 16] + i * KL % 16 * ts + vlane);
+        }
+    };
+    auto start = [&](const Segment &sg) {
+        if (sg.first >= sg.stop) return;
+        runs.start(A.c, (uint32_t)sg.first / 16, sg.end);
+        load_keys(sg.it);
+        load_values();
+    };
+    Segment sg = segment();
+    start(sg);
+
+    // tile after tile until the share is used up; the next one's first loads go out before this one's end
+    for (;;) {
+    const Item it = sg.it;
     const uint32_t r = it.rt * 16 + col, rows = (uint32_t)it.nq * A.group;
     const bool valid = r < rows;
     const uint32_t tok = valid ? r / A.group : 0, x = it.h * A.group + (valid ? r - tok * A.group : 0);
     const uint64_t row = (uint64_t)(it.r0 + (int32_t)tok);
-    const int32_t sees = valid ? min(max(it.len - it.nq + (int32_t)tok + 1, 0), end) : 0;
+    const int32_t sees = valid ? min(max(it.len - it.nq + (int32_t)tok + 1, 0), sg.end) : 0;
     const int32_t sees_min = __builtin_amdgcn_readfirstlane(sees);
     float c2 = A.scale * (C == kE4M3 && A.c.k_scale ? A.c.k_scale[it.h] : 1.0f) * 1.44269504088896340736f;
     const uint32_t flip = c2 < 0.0f ? 0x80000000u : 0u;
@@ -739,37 +817,8 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
     for (int i = 0; i < NB; ++i) o[i] = f32x4{0, 0, 0, 0};
     Row st{-INFINITY, 0.0f};
     uint8_t *const lds = sh + wave * G::WAVE;
-
-    const uint64_t head = it.h * A.c.head_stride;
-    Runs runs;
-    const int32_t share = (max(0, stop - first) + W * KEYS - 1) / (W * KEYS) * KEYS;  // keys of a wave
-    const int32_t wfirst = first + (int32_t)wave * share, wstop = min(stop, wfirst + share);
-    runs.start(A.c, (uint32_t)wfirst / 16, end);
-    Piece<C> kr[NR][NK], vr[NV];
-    // addresses: a scalar base for a run of keys or a load of values, and one offset a lane for each kind
-    const uint32_t ts = (uint32_t)A.c.token_stride * kSize<C>, klane = col * ts + g * PN * kSize<C>;
-    const uint32_t vlane = lane / (D / PN) * ts + lane % (D / PN) * PN * kSize<C>;
-    uint64_t base[NR];
-    auto load_keys = [&] {
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-            base[n] = runs.next(A.c, it, head) * kSize<C>;
-#pragma unroll
-            for (int s = 0; s < NK; ++s) kr[n][s].load((const uint8_t *)A.c.k + base[n] + klane + s * 4 * PN * kSize<C>);
-        }
-    };
-    auto load_values = [&] {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            constexpr int KL = 64 / (D / PN);  // keys a load
-            vr[i].load((const uint8_t *)A.c.v + base[i * KL / 16] + i * KL % 16 * ts + vlane);
-        }
-    };
+    const int32_t wfirst = sg.first, wstop = sg.stop;
     int32_t bad_at = -1;
-    if (wfirst < wstop) {
-        load_keys();
-        load_values();
-    }
     for (int32_t key0 = wfirst; key0 < wstop; key0 += KEYS) {
         f32x4 sc[NR];
 #pragma unroll
@@ -783,7 +832,7 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (key0 + KEYS < wstop) load_keys();
+        if (key0 + KEYS < wstop) load_keys(it);
         // values into the wave's tile; what is behind the sequence's end counts as 0
         const bool masked = key0 + KEYS > sees_min;
         if (masked) {
@@ -860,6 +909,13 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
     }
     if (bad_at >= 0) add_not_finite<C, D, false>(A.c, it, bad_at, min(wstop, it.len), sees, o);
 
+    const Segment done = sg;
+    const bool more = advance(sg.take);
+    if (more) {
+        sg = segment();
+        start(sg);
+    }
+
     // the waves' sums
     const uint32_t tid = thread_id(), ecol = tid & 15, eg = tid >> 4 & 3;
     st.l += __shfl_xor(st.l, 16);
@@ -873,7 +929,7 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
     for (int i = 0; i < NB; ++i) *(f32x4 *)(mine + ecol * D + ((i * 16 + eg * 4) ^ ((ecol & 7) << 2))) = o[i];
     __syncthreads();
     // a workgroup's share starts with at most one tile's end and ends with at most one tile's start
-    float *const part = (float *)A.work + (2 * (uint64_t)blockIdx.x + (pl.unit0 == 0)) * G::SLOT;
+    float *const part = (float *)A.work + (2 * (uint64_t)blockIdx.x + done.opens) * G::SLOT;
     const float vs = C == kE4M3 && A.c.v_scale ? A.c.v_scale[it.h] : 1.0f;
 #pragma unroll
     for (int e = 0; e < 16 * D / 4 / (64 * W); ++e) {
@@ -894,7 +950,7 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = __builtin_fmaf(z[i], f, y[i]);
         }
-        if (!whole) {
+        if (!done.whole) {
             *(f32x4 *)(part + rr * D + d) = y;
             if (d == 0) {
                 part[16 * D + rr] = m;
@@ -906,23 +962,8 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
                       it.len - it.nq + (int32_t)t + 1 > 0 ? vs / l : 0.0f);
         }
     }
-    left -= take;
-    if (!left) return;
-    pl.unit0 = 0;
-    if (++pl.h == A.c.kv_heads) {
-        pl.h = 0;
-        if (++pl.j == pl.tiles) {
-            pl.j = 0;
-            do {
-                if (++pl.b == A.c.n) return;
-                const Seq s = sequence(A.c, pl.b);
-                pl.s = Seq{__builtin_amdgcn_readfirstlane(s.r0), __builtin_amdgcn_readfirstlane(s.nq),
-                           __builtin_amdgcn_readfirstlane(s.len)};
-                pl.tiles = tiles_of<G::BM>(pl.s, A.group);
-            } while (!pl.tiles);
-            pl.units = units_of(pl.s, unit, slots);
-        }
-    }
+    if (!more) return;
+    __syncthreads();
     }
 }
 
