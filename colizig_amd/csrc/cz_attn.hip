@@ -47,14 +47,6 @@ __device__ __forceinline__ Seq sequence(const AttnCache &c, uint32_t b) {
     return s;
 }
 
-// A page number of the table; one outside the cache is flagged and read as 0.
-__device__ __forceinline__ uint32_t page_at(const AttnCache &c, uint32_t b, uint32_t i) {
-    // uniform: a scalar load
-    const uint32_t p = (uint32_t)*(const __attribute__((address_space(4))) int32_t *)(uintptr_t)(c.table + (uint64_t)b * c.max_pages + i);
-    if (p < c.pages) return p;
-    flag(c.err, kAttnBadPage);
-    return 0;
-}
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -595,27 +587,41 @@ __device__ __forceinline__ void tile_keys(const Item &it, uint32_t group, int32_
     *parts = max(1u, (units + *per - 1) / *per);
 }
 
-// Element offsets of a sequence's runs of 16 keys, one after the other; past the
-// last key the last run again (its loads stay in bounds, its keys are masked).
+// A sequence's runs of 16 keys, one after the other; past the last key the last run
+// again (its loads stay in bounds, its keys are masked).  Page numbers come by
+// scalar loads: fetch() asks for N runs' at once and place() takes them later, so
+// that the look-up of a tile's pages goes on under the tile before it.
+template <int N>
 struct Runs {
-    uint32_t j, slot, last;  // next run's page index and slot; runs left
-    __device__ __forceinline__ void start(const AttnCache &c, uint32_t run, int32_t keys) {
-        const uint32_t n = (uint32_t)(keys + 15) / 16, at = min(run, n ? n - 1 : 0);
-        j = at * 16 / c.page_size;
-        slot = at * 16 - j * c.page_size;
-        last = n ? n - 1 - at : 0;
+    const int32_t *table;
+    uint32_t j, slot, last;        // the next run's page index and slot; runs left after it
+    uint32_t page[N], at[N];       // of the runs asked for
+    __device__ __forceinline__ void start(const AttnCache &c, uint32_t b, uint32_t run, int32_t keys) {
+        const uint32_t n = (uint32_t)(keys + 15) / 16, first = min(run, n ? n - 1 : 0);
+        table = c.table + (uint64_t)b * c.max_pages;
+        j = first * 16 / c.page_size;
+        slot = first * 16 - j * c.page_size;
+        last = n ? n - 1 - first : 0;
+        fetch(c);
     }
-    __device__ __forceinline__ uint64_t next(const AttnCache &c, const Item &it, uint64_t head) {
-        const uint64_t at = page_at(c, it.b, j) * c.page_stride + slot * c.token_stride + head;
-        if (last) {
-            --last;
-            slot += 16;
-            if (slot >= c.page_size) {
-                slot = 0;
-                ++j;
+    __device__ __forceinline__ void fetch(const AttnCache &c) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            page[i] = (uint32_t)*(const __attribute__((address_space(4))) int32_t *)(uintptr_t)(table + j);
+            at[i] = slot;
+            const uint32_t next = slot + 16, wrap = next >= c.page_size;
+            if (last) {
+                --last;
+                slot = wrap ? 0 : next;
+                j += wrap;
             }
         }
-        return at;
+    }
+    // Element offset of run i's first key; a page outside the cache is noted and read as page 0.
+    __device__ __forceinline__ uint64_t place(const AttnCache &c, uint64_t head, int i, bool *bad) const {
+        const bool in = page[i] < c.pages;
+        *bad |= !in;
+        return (in ? page[i] : 0) * c.page_stride + at[i] * c.token_stride + head;
     }
 };
 
@@ -666,11 +672,12 @@ __device__ __forceinline__ void add_not_finite(const AttnCache &c, const Item &i
                                                V (&o)[NB]) {
     constexpr int M = W32 ? 32 : 16;
     const uint32_t d0 = (thread_id() & 63) / M * 4;
-    Runs runs;
-    runs.start(c, (uint32_t)from / 16, to);
+    Runs<1> runs;
+    bool bad;  // (noted before)
+    runs.start(c, it.b, (uint32_t)from / 16, to);
 #pragma unroll 1
-    for (int32_t run = from / 16 * 16; run < to; run += 16) {
-        const uint64_t base = runs.next(c, it, it.h * c.head_stride) + d0;
+    for (int32_t run = from / 16 * 16; run < to; run += 16, runs.fetch(c)) {
+        const uint64_t base = runs.place(c, it.h * c.head_stride, 0, &bad) + d0;
 #pragma unroll 1
         for (int32_t key = max(run, from); key < min(run + 16, to); ++key) {
             const uint64_t at = base + (uint64_t)(key - run) * c.token_stride;
@@ -764,7 +771,8 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
         return true;
     };
 
-    Runs runs;
+    Runs<NR> runs;
+    bool bad_page = false;
     Piece<C> kr[NR][NK], vr[NV];
     // addresses: a scalar base for a run of keys or a load of values, and one offset a lane for each kind
     const uint32_t ts = (uint32_t)A.c.token_stride * kSize<C>, klane = col * ts + g * PN * kSize<C>;
@@ -773,10 +781,11 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
     auto load_keys = [&](const Item &it) {
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-            base[n] = runs.next(A.c, it, it.h * A.c.head_stride) * kSize<C>;
+            base[n] = runs.place(A.c, it.h * A.c.head_stride, n, &bad_page) * kSize<C>;
 #pragma unroll
             for (int s = 0; s < NK; ++s) kr[n][s].load_once((const uint8_t *)A.c.k + base[n] + klane + s * 4 * PN * kSize<C>);
         }
+        runs.fetch(A.c);
     };
     auto load_values = [&] {
 #pragma unroll
@@ -787,7 +796,7 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
     };
     auto start = [&](const Segment &sg) {
         if (sg.first >= sg.stop) return;
-        runs.start(A.c, (uint32_t)sg.first / 16, sg.end);
+        runs.start(A.c, sg.it.b, (uint32_t)sg.first / 16, sg.end);
         load_keys(sg.it);
         load_values();
     };
@@ -962,9 +971,10 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
                       it.len - it.nq + (int32_t)t + 1 > 0 ? vs / l : 0.0f);
         }
     }
-    if (!more) return;
+    if (!more) break;
     __syncthreads();
     }
+    if (bad_page) flag(A.c.err, kAttnBadPage);
 }
 
 // Joins the parts of a tile.  LD lanes read LD * 4 numbers of a part's row; a
@@ -1097,8 +1107,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
     Row st{-INFINITY, 0.0f};
 
     const uint64_t head = it.h * A.c.head_stride;
-    Runs runs;
-    runs.start(A.c, (uint32_t)(first / 16), end);
+    Runs<BK / 16> runs;
+    bool bad_page = false;
+    if (first < stop) runs.start(A.c, it.b, (uint32_t)(first / 16), end);
     Piece<C> kr[NL], vr[NL];
     // thread t's pieces are of keys t / (D / PN) + STEP i, so a wave's are of one run
     const uint32_t ch = threadIdx.x % (D / PN), tkey = threadIdx.x / (D / PN);
@@ -1108,7 +1119,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
     auto load = [&] {
         uint64_t base[BK / 16];
 #pragma unroll
-        for (int i = 0; i < BK / 16; ++i) base[i] = runs.next(A.c, it, head) * kSize<C>;
+        for (int i = 0; i < BK / 16; ++i) base[i] = runs.place(A.c, head, i, &bad_page) * kSize<C>;
+        runs.fetch(A.c);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             // with 16 keys or more from piece to piece, waves are of different runs
@@ -1232,6 +1244,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
         __syncthreads();
     }
 
+    if (bad_page) flag(A.c.err, kAttnBadPage);
     if (__syncthreads_or(bad))
         add_not_finite<C, D, true>(A.c, it, max(first, cut / BK * BK), min(stop, it.len), sees, o);
     st.l += __shfl_xor(st.l, 32);
