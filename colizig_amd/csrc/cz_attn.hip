@@ -246,6 +246,15 @@ __device__ __forceinline__ void store8(uint8_t *p, const float (&y)[8]) {
     }
 }
 
+__device__ __forceinline__ void floats8(const float *p, float (&x)[8]) {
+    const f32x4 a = *(const f32x4 *)p, b = *(const f32x4 *)(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[i] = a[i];
+        x[4 + i] = b[i];
+    }
+}
+
 // ---- append -------------------------------------------------------------------
 // Head vectors (the query's into q_out, then the keys, then the values) over groups
 // of D / 8 lanes, 8 neighbouring numbers a lane, so that a vector moves in 16-byte
@@ -311,10 +320,8 @@ __global__ __launch_bounds__(256) void k_append(AppendArgs A) {
         // the lane's angles: numbers d < dims/2 turn with d + dims/2
         if (turns) {
             const float *p = A.rope + (uint64_t)pos * A.dims + (lower ? d0 : d0 - half);
-            *(f32x4 *)cs = *(const f32x4 *)p;
-            *(f32x4 *)(cs + 4) = *(const f32x4 *)(p + 4);
-            *(f32x4 *)sn = *(const f32x4 *)(p + half);
-            *(f32x4 *)(sn + 4) = *(const f32x4 *)(p + half + 4);
+            floats8(p, cs);
+            floats8(p + half, sn);
             if (lower)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sn[i] = -sn[i];
@@ -323,14 +330,8 @@ __global__ __launch_bounds__(256) void k_append(AppendArgs A) {
         if (!paged) flag(A.c.err, kAttnBadPage);
         to = page * A.c.page_stride + (pos - pi * A.c.page_size) * A.c.token_stride;
     }
-    if (A.q_norm) {
-        *(f32x4 *)wq = *(const f32x4 *)(A.q_norm + d0);
-        *(f32x4 *)(wq + 4) = *(const f32x4 *)(A.q_norm + d0 + 4);
-    }
-    if (A.k_norm) {
-        *(f32x4 *)wk = *(const f32x4 *)(A.k_norm + d0);
-        *(f32x4 *)(wk + 4) = *(const f32x4 *)(A.k_norm + d0 + 4);
-    }
+    if (A.q_norm) floats8(A.q_norm + d0, wq);
+    if (A.k_norm) floats8(A.k_norm + d0, wk);
     const int other = (int)((turns ? (lower ? lane + half / 8 : lane - half / 8) : lane) * 4);
 
     for (uint32_t x0 = xs; x0 < heads; x0 += UNROLL * xstep) {  // (the bound is over a group: its lanes stay together)
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(256) void k_append(AppendArgs A) {
                 for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(y[i], y[i], ss);
 #pragma unroll
                 for (int m = LV / 2; m; m >>= 1) ss += __shfl_xor(ss, m);
-                const float r = 1.0f / __builtin_sqrtf(ss / D + A.eps);
+                const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(ss, 1.0f / D, A.eps));
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = y[i] * r * (isq ? wq[i] : wk[i]);
             }
