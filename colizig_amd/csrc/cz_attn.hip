@@ -279,7 +279,7 @@ __global__ __launch_bounds__(256) void k_append(AppendArgs A) {
             const bool isq = x < A.q_heads, isk = x < A.q_heads + A.c.kv_heads;
             const uint32_t h = isq ? x : isk ? x - A.q_heads : x - A.q_heads - A.c.kv_heads;
             const uint64_t at = (uint64_t)t * (isq ? A.q_stride : isk ? A.k_stride : A.v_stride) + h * D + gl * 8;
-            in[u].load((const uint8_t *)(isq ? A.q : isk ? A.k : A.v) + at * kSize<R>);
+            in[u].load_once((const uint8_t *)(isq ? A.q : isk ? A.k : A.v) + at * kSize<R>);
         }
     };
     load(xs);
@@ -449,71 +449,6 @@ struct Item {
     int32_t r0, nq, len;
 };
 
-// Item `idx` of a call, found by every wave for itself.  Row tiles of BM rows,
-// keys in units of UNIT.  Where there are fewer tiles than `slots` workgroups
-// (0: never), each sequence's tiles are cut into parts of at most C units, C the
-// smallest that keeps the parts within `slots`: ragged lengths share the chip
-// evenly.  Order: sequence, tile (the last first: it sees most), part, key head -
-// heads innermost, so that a head's workgroups stay on the same XCDs' L2.
-// JOIN: an item per tile instead of one per part.
-template <int BM, int UNIT, bool JOIN>
-__device__ __forceinline__ bool find_item(const AttnCache &c, uint32_t group, uint32_t slots, uint32_t idx, Item &it) {
-    const uint32_t lane = threadIdx.x & 63;
-    Seq s{0, 0, 0};  // of the lane's sequence; up to 64 are read once
-    auto read = [&](uint32_t b0) {
-        s = Seq{0, 0, 0};
-        if (b0 + lane < c.n) s = sequence(c, b0 + lane);
-    };
-    read(0);
-    uint32_t C = 0xffffffffu;
-    if (slots) {
-        float total = 0;
-        uint32_t tiles = 0;
-        for (uint32_t b0 = 0;;) {
-            const uint32_t t = ((uint32_t)s.nq * group + BM - 1) / BM;
-            tiles += t;
-            total += (float)t * (float)((s.len + UNIT - 1) / UNIT);
-            if ((b0 += 64) >= c.n) break;
-            read(b0);
-        }
-        total = lane_of(wave_scan(total), 63);
-        tiles = lane_of(wave_scan(tiles), 63);
-        const uint32_t room = slots / c.kv_heads;
-        if (tiles < room) C = max(1u, (uint32_t)__builtin_ceilf(total / (float)(room - tiles) * 1.00001f));
-        if (c.n > 64) read(0);
-    }
-    uint32_t base = 0, slot0 = 0;
-    for (uint32_t b0 = 0; b0 < c.n; b0 += 64) {
-        if (b0) read(b0);
-        uint32_t t = ((uint32_t)s.nq * group + BM - 1) / BM, parts = 1;
-        if (C != 0xffffffffu) parts = max(1u, ((uint32_t)(s.len + UNIT - 1) / UNIT + C - 1) / C);
-        const uint32_t all = t * parts * c.kv_heads, mine = JOIN ? t * c.kv_heads : all;
-        const uint32_t end = wave_scan(mine), send = JOIN ? wave_scan(all) : 0;
-        const uint64_t hit = __ballot(base + end > idx);
-        if (hit) {
-            const int w = __ffsll((unsigned long long)hit) - 1;
-            it.b = b0 + w;
-            it.r0 = __builtin_amdgcn_readlane(s.r0, w);
-            it.nq = __builtin_amdgcn_readlane(s.nq, w);
-            it.len = __builtin_amdgcn_readlane(s.len, w);
-            it.parts = __builtin_amdgcn_readlane(parts, w);
-            t = __builtin_amdgcn_readlane(t, w);
-            const uint32_t rel = idx - (base + __builtin_amdgcn_readlane(end - mine, w));
-            const uint32_t per = JOIN ? c.kv_heads : it.parts * c.kv_heads;
-            const uint32_t j = rel / per, rem = rel - j * per;
-            it.rt = t - 1 - j;
-            it.part = rem / c.kv_heads;
-            it.h = rem - it.part * c.kv_heads;
-            // where the tile's first part's sums are
-            it.slot = JOIN ? slot0 + __builtin_amdgcn_readlane(send - all, w) + j * it.parts * c.kv_heads + it.h : idx;
-            return true;
-        }
-        base += __builtin_amdgcn_readlane(end, 63);
-        if (JOIN) slot0 += __builtin_amdgcn_readlane(send, 63);
-    }
-    return false;
-}
-
 // A share of a call's work: all tiles' units of `unit` keys, in the order sequence,
 // tile (the last first), key head, unit, dealt out evenly to `slots` workgroups
 // whatever the lengths are; a tile that several of them share is joined from their
@@ -578,6 +513,126 @@ __device__ __forceinline__ bool find_place(const AttnCache &c, uint32_t group, u
     return false;
 }
 
+// Item `idx` of a call, found by every wave for itself.  Row tiles of BM rows,
+// keys in units of UNIT.  Where there are fewer tiles than workgroups on the chip (half
+// of `slots`; 0: never), each sequence's tiles are cut into parts of at most C units:
+// ragged lengths share the chip evenly.  Order: sequence, tile (the last first: it sees most), part, key head -
+// heads innermost, so that a head's workgroups stay on the same XCDs' L2.
+// JOIN: an item per tile instead of one per part.
+template <int BM, int UNIT, bool JOIN>
+__device__ __forceinline__ bool find_item(const AttnCache &c, uint32_t group, uint32_t slots, uint32_t idx, Item &it) {
+    const uint32_t lane = threadIdx.x & 63;
+    Seq s{0, 0, 0};  // of the lane's sequence; up to 64 are read once
+    auto read = [&](uint32_t b0) {
+        s = Seq{0, 0, 0};
+        if (b0 + lane < c.n) s = sequence(c, b0 + lane);
+    };
+    read(0);
+    uint32_t C = 0xffffffffu;
+    if (slots) {
+        float total = 0;
+        uint32_t tiles = 0;
+        for (uint32_t b0 = 0;;) {
+            const uint32_t t = tiles_of<BM>(s, group);
+            tiles += t;
+            total += (float)t * (float)((s.len + UNIT - 1) / UNIT);
+            if ((b0 += 64) >= c.n) break;
+            read(b0);
+        }
+        total = lane_of(wave_scan(total), 63);
+        tiles = lane_of(wave_scan(tiles), 63);
+        // Parts for one round of the chip, or for two: 196 tiles of 325 units make 392 parts of 163 in one
+        // round, which leaves a quarter of it idle, or 980 of 65 in two (398 and 361 us).
+        float best = 0;
+        for (uint32_t k = 1; k <= 2; ++k) {
+            const uint32_t room = k * (slots / 2) / c.kv_heads;
+            if (tiles >= room) continue;
+            const uint32_t Ck = max(1u, (uint32_t)__builtin_ceilf(total / (float)(room - tiles) * 1.00001f));
+            uint32_t sum = 0, longest = 0;
+            for (uint32_t b0 = 0; b0 < c.n; b0 += 64) {
+                if (c.n > 64) read(b0);
+                const uint32_t u = (uint32_t)(s.len + UNIT - 1) / UNIT, parts = max(1u, (u + Ck - 1) / Ck);
+                const uint32_t t = tiles_of<BM>(s, group);
+                sum += t * parts;
+                longest = max(longest, t ? (u + parts - 1) / parts : 0);
+            }
+            sum = lane_of(wave_scan(sum), 63) * c.kv_heads;
+#pragma unroll
+            for (int m = 32; m; m >>= 1) longest = max(longest, (uint32_t)__shfl_xor((int)longest, m));
+            // (a part's start and end cost about two units)
+            const float cost = __builtin_ceilf((float)sum / (float)(slots / 2)) * (float)(longest + 2);
+            if (k == 1 || C == 0xffffffffu || cost < best) {
+                best = cost;
+                C = Ck;
+            }
+        }
+        if (c.n > 64) read(0);
+    }
+    if (!JOIN && !slots && c.n <= 64) {
+        // No parts: the tiles with the most units first, whichever sequence they are of, so that the last
+        // ones to start are short.  reach(U): tiles of the lane's sequence that have at least U units, which
+        // are its last ones: the largest U that idx tiles or fewer reach is that of tile idx.
+        const uint32_t t = tiles_of<BM>(s, group);
+        const int32_t past = s.len - s.nq;
+        auto reach = [&](uint32_t U) {
+            const int32_t tok = (int32_t)((U - 1) * UNIT) - past;  // a last row of this token or later
+            if (U == 1 || tok <= 0) return t;                      // (a tile that sees nothing is written too)
+            return tok >= s.nq ? 0u : t - ((uint32_t)tok * group + BM) / BM + 1;
+        };
+        auto total = [&](uint32_t U) { return lane_of(wave_scan(reach(U)), 63) * c.kv_heads; };
+        if (idx >= total(1)) return false;
+        uint32_t lo = 1, hi = (c.max_pages * c.page_size + UNIT - 1) / UNIT + 1;  // total(lo) > idx >= total(hi)
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (total(mid) > idx) lo = mid; else hi = mid;
+        }
+        const uint32_t more = reach(lo + 1), mine = reach(lo) - more;  // tiles of exactly lo units
+        const uint32_t rel = idx - total(lo + 1), end = wave_scan(mine) * c.kv_heads;
+        const int w = __ffsll((unsigned long long)__ballot(end > rel)) - 1;
+        const uint32_t at = rel - lane_of(end - mine * c.kv_heads, w), j = at / c.kv_heads;
+        it.b = w;
+        it.r0 = lane_of(s.r0, w);
+        it.nq = lane_of(s.nq, w);
+        it.len = lane_of(s.len, w);
+        it.parts = 1;
+        it.rt = lane_of(t - 1 - more, w) - j;
+        it.part = 0;
+        it.h = at - j * c.kv_heads;
+        it.slot = idx;
+        return true;
+    }
+    uint32_t base = 0, slot0 = 0;
+    for (uint32_t b0 = 0; b0 < c.n; b0 += 64) {
+        if (b0) read(b0);
+        uint32_t t = ((uint32_t)s.nq * group + BM - 1) / BM, parts = 1;
+        if (C != 0xffffffffu) parts = max(1u, ((uint32_t)(s.len + UNIT - 1) / UNIT + C - 1) / C);
+        const uint32_t all = t * parts * c.kv_heads, mine = JOIN ? t * c.kv_heads : all;
+        const uint32_t end = wave_scan(mine), send = JOIN ? wave_scan(all) : 0;
+        const uint64_t hit = __ballot(base + end > idx);
+        if (hit) {
+            const int w = __ffsll((unsigned long long)hit) - 1;
+            it.b = b0 + w;
+            it.r0 = __builtin_amdgcn_readlane(s.r0, w);
+            it.nq = __builtin_amdgcn_readlane(s.nq, w);
+            it.len = __builtin_amdgcn_readlane(s.len, w);
+            it.parts = __builtin_amdgcn_readlane(parts, w);
+            t = __builtin_amdgcn_readlane(t, w);
+            const uint32_t rel = idx - (base + __builtin_amdgcn_readlane(end - mine, w));
+            const uint32_t per = JOIN ? c.kv_heads : it.parts * c.kv_heads;
+            const uint32_t j = rel / per, rem = rel - j * per;
+            it.rt = t - 1 - j;
+            it.part = rem / c.kv_heads;
+            it.h = rem - it.part * c.kv_heads;
+            // where the tile's first part's sums are
+            it.slot = JOIN ? slot0 + __builtin_amdgcn_readlane(send - all, w) + j * it.parts * c.kv_heads + it.h : idx;
+            return true;
+        }
+        base += __builtin_amdgcn_readlane(end, 63);
+        if (JOIN) slot0 += __builtin_amdgcn_readlane(send, 63);
+    }
+    return false;
+}
+
 // Keys that the tile's last row sees, and the units of them that each part takes.
 template <int BM, int UNIT>
 __device__ __forceinline__ void tile_keys(const Item &it, uint32_t group, int32_t *end, uint32_t *per, uint32_t *parts) {
@@ -588,21 +643,26 @@ __device__ __forceinline__ void tile_keys(const Item &it, uint32_t group, int32_
     *parts = max(1u, (units + *per - 1) / *per);
 }
 
-// A sequence's runs of 16 keys, one after the other; past the last key the last run
-// again (its loads stay in bounds, its keys are masked).  Page numbers come by
-// scalar loads: fetch() asks for N runs' at once and place() takes them later, so
-// that the look-up of a tile's pages goes on under the tile before it.
-template <int N>
+// Runs of 16 keys of a sequence: N neighbours at a time, STEP runs from one time to
+// the next; past the last key the last run again, or the one before (its loads stay in
+// bounds, its keys are masked).  Page numbers come by scalar loads: fetch() asks for
+// N runs' and place() takes them later, so that the look-up of a tile's pages goes on
+// under the tile before it.
+template <int N, int STEP = N>
 struct Runs {
     const int32_t *table;
-    uint32_t j, slot, last;        // the next run's page index and slot; runs left after it
+    uint32_t j, slot, next, last;  // page index and slot of the next run, its number, and the last one's
+    uint32_t step_j, step_slot;    // STEP - N runs further, in pages and slots
     uint32_t page[N], at[N];       // of the runs asked for
     __device__ __forceinline__ void start(const AttnCache &c, uint32_t b, uint32_t run, int32_t keys) {
-        const uint32_t n = (uint32_t)(keys + 15) / 16, first = min(run, n ? n - 1 : 0);
+        const uint32_t n = (uint32_t)(keys + 15) / 16;
+        last = n ? n - 1 : 0;
+        next = min(run, last);
         table = c.table + (uint64_t)b * c.max_pages;
-        j = first * 16 / c.page_size;
-        slot = first * 16 - j * c.page_size;
-        last = n ? n - 1 - first : 0;
+        j = next * 16 / c.page_size;
+        slot = next * 16 - j * c.page_size;
+        step_j = (STEP - N) * 16 / c.page_size;
+        step_slot = (STEP - N) * 16 - step_j * c.page_size;
         fetch(c);
     }
     __device__ __forceinline__ void fetch(const AttnCache &c) {
@@ -610,11 +670,19 @@ struct Runs {
         for (int i = 0; i < N; ++i) {
             page[i] = (uint32_t)*(const __attribute__((address_space(4))) int32_t *)(uintptr_t)(table + j);
             at[i] = slot;
-            const uint32_t next = slot + 16, wrap = next >= c.page_size;
-            if (last) {
-                --last;
-                slot = wrap ? 0 : next;
-                j += wrap;
+            const uint32_t far = i + 1 == N ? 1 + STEP - N : 1;  // to the run after it
+            if (next + far <= last) {
+                next += far;
+                slot += 16 + (far > 1 ? step_slot : 0);
+                j += far > 1 ? step_j : 0;
+                if (slot >= c.page_size) {
+                    slot -= c.page_size;
+                    ++j;
+                }
+                if (far > 1 && slot >= c.page_size) {
+                    slot -= c.page_size;
+                    ++j;
+                }
             }
         }
     }
@@ -1062,7 +1130,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots, u
 template <uint32_t R, uint32_t C, int D>
 struct TileCfg {
     static constexpr int QT = kTerms<R>, KT = kTerms<C>, BM = 128;
-    static constexpr int BK = KT == 3 || D == 256 ? 32 : 64;
+    static constexpr int BK = KT == 3 || D == 256 || (QT == 3 && D == 128) ? 32 : 64;
     static constexpr int PLANE = BK * D * 2, HALF = PLANE * KT;       // bytes of a tile's K, and of its V
     static constexpr int BUF = 4 * HALF <= 128 * 1024 ? 2 : 1;
     static constexpr int SLOT = BM * (D + 2);
@@ -1108,33 +1176,21 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
     Row st{-INFINITY, 0.0f};
 
     const uint64_t head = it.h * A.c.head_stride;
-    Runs<BK / 16> runs;
+    // A wave stages a quarter of the tile's keys, all of one run.
+    constexpr int KW = BK / 4, KL = 64 / (D / PN);  // keys a wave, and a load
+    Runs<1, BK / 16> runs;
     bool bad_page = false;
-    if (first < stop) runs.start(A.c, it.b, (uint32_t)(first / 16), end);
+    if (first < stop) runs.start(A.c, it.b, (uint32_t)first / 16 + wave * KW / 16, end);
     Piece<C> kr[NL], vr[NL];
-    // thread t's pieces are of keys t / (D / PN) + STEP i, so a wave's are of one run
-    const uint32_t ch = threadIdx.x % (D / PN), tkey = threadIdx.x / (D / PN);
-    const uint32_t voff = ((tkey & 15) * (uint32_t)A.c.token_stride + ch * PN) * kSize<C>;
-    constexpr int STEP = 256 / (D / PN);  // keys from one piece of a thread to its next
-    const uint32_t vnext = STEP < 16 ? STEP * (uint32_t)A.c.token_stride * kSize<C> : 0;
+    const uint32_t ch = lane % (D / PN), tkey = wave * KW + lane / (D / PN), ts = (uint32_t)A.c.token_stride * kSize<C>;
+    const uint32_t voff = (tkey & 15) * ts + ch * PN * kSize<C>;
     auto load = [&] {
-        uint64_t base[BK / 16];
-#pragma unroll
-        for (int i = 0; i < BK / 16; ++i) base[i] = runs.place(A.c, head, i, &bad_page) * kSize<C>;
+        const uint64_t at = runs.place(A.c, head, 0, &bad_page) * kSize<C>;
         runs.fetch(A.c);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            // with 16 keys or more from piece to piece, waves are of different runs
-            constexpr int PER = STEP >= 16 ? STEP / 16 : 1;
-            uint64_t at = base[STEP >= 16 ? i * PER : i * STEP / 16];
-            if constexpr (PER > 1) {
-                const uint32_t run = wave * 64 / (D / PN) / 16;
-#pragma unroll
-                for (int n = 1; n < PER; ++n) at = run == n ? base[i * PER + n] : at;
-            }
-            const uint32_t off = voff + (STEP < 16 && i * STEP % 16 ? vnext : 0);
-            kr[i].load((const uint8_t *)A.c.k + at + off);
-            vr[i].load((const uint8_t *)A.c.v + at + off);
+            kr[i].load((const uint8_t *)A.c.k + at + i * KL * ts + voff);
+            vr[i].load((const uint8_t *)A.c.v + at + i * KL * ts + voff);
         }
     };
     // masks cut through the workgroup's tiles from here on
@@ -1144,7 +1200,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
         if (key0 + BK > cut) {
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
-                if (key0 + (int32_t)(i * STEP + tkey) >= it.len) vr[i].zero();
+                if (key0 + (int32_t)(i * KL + tkey) >= it.len) vr[i].zero();
                 bad |= vr[i].clean();
             }
         }
@@ -1155,7 +1211,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
                 bf8 k[KT], v[KT];
                 kr[i].terms(u, k);
                 vr[i].terms(u, v);
-                const uint32_t at = lds_at<D>(tkey, ch * SUB + u) + i * STEP * D * 2;
+                const uint32_t at = lds_at<D>(i * KL + tkey, ch * SUB + u);
 #pragma unroll
                 for (int t = 0; t < KT; ++t) {
                     *(bf8 *)(to + t * G::PLANE + at) = k[t];
@@ -1175,9 +1231,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
         if (more) load();
         const uint8_t *const ks = sh + buf * 2 * G::HALF, *const vs = ks + G::HALF;
         if (key0 < sees_max) {
+            const bool masked = key0 + BK > sees_min;
+            const float cc = masked ? 1.0f : c2;
             f32x16 sc[NN];
-#pragma unroll
-            for (int n = 0; n < NN; ++n) {
+            bf8 pt[BK / 16][QT];
+            float mu;
+            // scores of 32 keys
+            auto scores = [&](int n) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sc[n][e] = 0.0f;
 #pragma unroll
@@ -1187,45 +1247,37 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
                     for (int t = 0; t < KT; ++t) k[t] = *(const bf8 *)(ks + t * G::PLANE + lds_at<D>(n * 32 + col, s * 2 + g));
                     sc[n] = product<KT, QT>(k, q[s], sc[n], mfma32);
                 }
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            float cc = c2;
-            const bool masked = key0 + BK > sees_min;
-            if (masked) {
-#pragma unroll
-                for (int n = 0; n < NN; ++n)
+            };
+            // their mask and maximum; what was summed so far is scaled down where that rises
+            auto largest = [&](int n) {
+                if (masked)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         sc[n][e] = key0 + n * 32 + (e / 4) * 8 + (int32_t)g * 4 + e % 4 < sees ? sc[n][e] * c2 : -INFINITY;
-                cc = 1.0f;
-            }
-            float mx = sc[0][0];
+                float m[4];
 #pragma unroll
-            for (int n = 0; n < NN; ++n)
+                for (int e = 0; e < 4; ++e) m[e] = fmaxf(fmaxf(sc[n][e], sc[n][e + 4]), fmaxf(sc[n][e + 8], sc[n][e + 12]));
+                const float mx = across32(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))) * cc;
+                if (__any(mx > st.m + 8.0f)) {
+                    const float mn = fmaxf(st.m, mx), f = exp2_hw(st.m - finite_max(mn));
+                    st.l *= f;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[n][e]);
-            mx = across32(mx) * cc;
-            if (__any(mx > st.m + 8.0f)) {
-                const float mn = fmaxf(st.m, mx), f = exp2_hw(st.m - finite_max(mn));
-                st.l *= f;
-#pragma unroll
-                for (int i = 0; i < NB; ++i) o[i] *= f;
-                st.m = mn;
-            }
-            const float mu = finite_max(st.m);
-            // 16 keys at a time: weights, then their products
-            const uint32_t tk = g * 4 + ((lane & 15) >> 2), tc = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), tb = (lane & 1) * 8;
-#pragma unroll
-            for (int n = 0; n < BK / 16; ++n) {
+                    for (int i = 0; i < NB; ++i) o[i] *= f;
+                    st.m = mn;
+                }
+                mu = finite_max(st.m);
+            };
+            // weights of 16 keys
+            auto weights = [&](int n) {
                 float p[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    p[i] = exp2_hw(__builtin_fmaf(sc[n / 2][(n % 2) * 8 + i], cc, -mu));
-                    st.l += p[i];
-                }
-                bf8 pt[QT];
-                split8<QT>(p, pt);
-                __builtin_amdgcn_sched_barrier(0);
+                for (int i = 0; i < 8; ++i) p[i] = exp2_hw(__builtin_fmaf(sc[n / 2][(n % 2) * 8 + i], cc, -mu));
+                st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                split8<QT>(p, pt[n]);
+            };
+            // their products with the values
+            const uint32_t tk = g * 4 + ((lane & 15) >> 2), tc = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), tb = (lane & 1) * 8;
+            auto values = [&](int n) {
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
                     bf8 v[KT];
@@ -1235,8 +1287,29 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
                         const u32x2 a = read_tr(vs, at), b = read_tr(vs, at + 8 * D * 2);
                         v[t] = __builtin_bit_cast(bf8, u32x4{a[0], a[1], b[0], b[1]});
                     }
-                    o[i] = product<KT, QT>(v, pt, o[i], mfma32);
+                    o[i] = product<KT, QT>(v, pt[n], o[i], mfma32);
                 }
+            };
+            // Matrix instructions beside vector ones that do not need them: the second half's scores with the first
+            // half's weights, the first half's values with the second half's weights.
+            scores(0);
+            largest(0);
+            if constexpr (NN == 2) {
+                scores(1);
+                weights(0);
+                weights(1);
+                largest(1);
+                weights(2);
+                weights(3);
+                values(0);
+                values(1);
+                values(2);
+                values(3);
+            } else {
+                weights(0);
+                weights(1);
+                values(0);
+                values(1);
             }
         }
         if (G::BUF == 1) __syncthreads();
@@ -1293,14 +1366,14 @@ void pick(uint32_t row_t, uint32_t cache_t, uint32_t dim, F &&f) {
 
 }  // namespace
 
-// Rows from which a workgroup takes eight.
+// Rows from which a workgroup takes four.
 constexpr uint32_t kAppendBlockRows = 2048;
 
 void launch_append(const AppendArgs &A, uint32_t row_t, uint32_t dim, hipStream_t st) {
     pick(row_t, A.c.dtype, dim, [&](auto r, auto c, auto d) {
         constexpr uint32_t groups = 256 / (d() / 8);
         if (A.c.rows >= kAppendBlockRows)
-            k_append<r(), c(), d(), 8><<<(A.c.rows + 7) / 8, 256, 0, st>>>(A);
+            k_append<r(), c(), d(), 4><<<(A.c.rows + 3) / 4, 256, 0, st>>>(A);
         else
             k_append<r(), c(), d(), 1><<<dim3(A.c.rows, (A.q_heads + 2 * A.c.kv_heads + groups - 1) / groups), 256, 0, st>>>(A);
     });
@@ -1322,7 +1395,7 @@ Plan plan(const AttnArgs &A, uint32_t dim) {
     // a sequence's last tile may be in part empty
     p.tiles = (uint32_t)std::min<uint64_t>(rows / bm + A.c.n, rows) * A.c.kv_heads;
     if (p.tile) {
-        p.slots = p.tiles < 512 ? 512 : 0;  // two workgroups on a CU
+        p.slots = p.tiles < 512 ? 1024 : 0;  // two workgroups on a CU, in up to two rounds
         p.unit = 0;
         return p;
     }
