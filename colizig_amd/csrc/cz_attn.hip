@@ -443,6 +443,10 @@ __device__ __forceinline__ T lane_of(T x, int lane) {
     return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
 }
 
+// The scratch: a line for how the work was divided, then the parts' sums.
+constexpr uint32_t kPlanFloats = 64;
+constexpr uint32_t kWhole = 0xffffffffu;  // no parts
+
 // One part of the work: keys of a row tile of a key head.
 struct Item {
     uint32_t b, rt, h, part, parts, slot;
@@ -464,10 +468,11 @@ __device__ __forceinline__ uint32_t units_of(const Seq &s, uint32_t unit, uint32
     return slots ? max(1u, ((uint32_t)s.len + unit - 1) / unit) : 1u;
 }
 
-// Unit idx * per (JOIN: tile idx), per being the share of a workgroup.
+// Unit idx * per (JOIN: tile idx), per being the share of a workgroup; JOIN: as the
+// first workgroup left it at `plan`.
 template <int BM, bool JOIN>
 __device__ __forceinline__ bool find_place(const AttnCache &c, uint32_t group, uint32_t slots, uint32_t unit, uint32_t idx,
-                                           uint32_t *per, Place &p) {
+                                           uint32_t *plan, uint32_t *per, Place &p) {
     const uint32_t lane = threadIdx.x & 63;
     Seq s{0, 0, 0};  // of the lane's sequence; up to 64 are read once
     auto read = [&](uint32_t b0) {
@@ -475,8 +480,8 @@ __device__ __forceinline__ bool find_place(const AttnCache &c, uint32_t group, u
         if (b0 + lane < c.n) s = sequence(c, b0 + lane);
     };
     read(0);
-    *per = 1;
-    if (slots) {
+    *per = JOIN ? *plan : 1;
+    if (!JOIN && slots) {
         uint32_t total = 0;
         for (uint32_t b0 = 0;;) {
             total += tiles_of<BM>(s, group) * units_of(s, unit, slots);
@@ -484,6 +489,7 @@ __device__ __forceinline__ bool find_place(const AttnCache &c, uint32_t group, u
             read(b0);
         }
         *per = max(1u, (lane_of(wave_scan(total), 63) * c.kv_heads + slots - 1) / slots);
+        if (blockIdx.x == 0) *plan = *per;
         if (c.n > 64) read(0);
     }
     const uint32_t want = JOIN ? idx : idx * *per;
@@ -520,7 +526,8 @@ __device__ __forceinline__ bool find_place(const AttnCache &c, uint32_t group, u
 // heads innermost, so that a head's workgroups stay on the same XCDs' L2.
 // JOIN: an item per tile instead of one per part.
 template <int BM, int UNIT, bool JOIN>
-__device__ __forceinline__ bool find_item(const AttnCache &c, uint32_t group, uint32_t slots, uint32_t idx, Item &it) {
+__device__ __forceinline__ bool find_item(const AttnCache &c, uint32_t group, uint32_t slots, uint32_t idx, uint32_t *plan,
+                                          Item &it) {
     const uint32_t lane = threadIdx.x & 63;
     Seq s{0, 0, 0};  // of the lane's sequence; up to 64 are read once
     auto read = [&](uint32_t b0) {
@@ -528,26 +535,41 @@ __device__ __forceinline__ bool find_item(const AttnCache &c, uint32_t group, ui
         if (b0 + lane < c.n) s = sequence(c, b0 + lane);
     };
     read(0);
-    uint32_t C = 0xffffffffu;
-    if (slots) {
-        float total = 0;
-        uint32_t tiles = 0;
+    uint32_t C = JOIN ? *plan : kWhole;
+    if (JOIN && C == kWhole) return false;
+    if (!JOIN && slots) {
+        float total = 0, seen = 0;  // units if each tile had the deepest's, and about what they have
+        uint32_t deepest = 0, tiles = 0;
         for (uint32_t b0 = 0;;) {
             const uint32_t t = tiles_of<BM>(s, group);
             tiles += t;
             total += (float)t * (float)((s.len + UNIT - 1) / UNIT);
+            seen += (float)t * ((float)s.len - 0.5f * (float)min(s.nq, s.len)) * (1.0f / UNIT);
+            deepest = max(deepest, t ? (uint32_t)(s.len + UNIT - 1) / UNIT : 0);
             if ((b0 += 64) >= c.n) break;
             read(b0);
         }
         total = lane_of(wave_scan(total), 63);
         tiles = lane_of(wave_scan(tiles), 63);
-        // Parts for one round of the chip, or for two: 196 tiles of 325 units make 392 parts of 163 in one
-        // round, which leaves a quarter of it idle, or 980 of 65 in two (398 and 361 us).
-        float best = 0;
+        auto largest = [](uint32_t x) {
+#pragma unroll
+            for (int m = 32; m; m >>= 1) x = max(x, (uint32_t)__shfl_xor((int)x, m));
+            return x;
+        };
+        // Whole tiles, or parts for one round of the chip, or for two, by units of time: a start and an end cost
+        // about two, joining ten, and beyond one round the work is spread evenly but for half a part.  196 tiles of
+        // 325 units make 392 parts of 163 in one round, which leaves a quarter of the chip idle, or 980 of 65 in two
+        // (398 and 361 us); 500 of up to 32 units are best left whole (62 us for 82 in parts).
+        const float chip = (float)(slots / 2);
+        seen = lane_of(wave_scan(seen), 63) * (float)c.kv_heads / chip;
+        auto time = [&](uint32_t items, uint32_t longest) {
+            return (float)items <= chip ? (float)(longest + 2) : seen + 2.0f * (float)items / chip + 0.5f * (float)longest;
+        };
+        float best = time(tiles * c.kv_heads, largest(deepest));
         for (uint32_t k = 1; k <= 2; ++k) {
             const uint32_t room = k * (slots / 2) / c.kv_heads;
             if (tiles >= room) continue;
-            const uint32_t Ck = max(1u, (uint32_t)__builtin_ceilf(total / (float)(room - tiles) * 1.00001f));
+            const uint32_t Ck = max(3u, (uint32_t)__builtin_ceilf(total / (float)(room - tiles) * 1.00001f));
             uint32_t sum = 0, longest = 0;
             for (uint32_t b0 = 0; b0 < c.n; b0 += 64) {
                 if (c.n > 64) read(b0);
@@ -556,19 +578,16 @@ __device__ __forceinline__ bool find_item(const AttnCache &c, uint32_t group, ui
                 sum += t * parts;
                 longest = max(longest, t ? (u + parts - 1) / parts : 0);
             }
-            sum = lane_of(wave_scan(sum), 63) * c.kv_heads;
-#pragma unroll
-            for (int m = 32; m; m >>= 1) longest = max(longest, (uint32_t)__shfl_xor((int)longest, m));
-            // (a part's start and end cost about two units)
-            const float cost = __builtin_ceilf((float)sum / (float)(slots / 2)) * (float)(longest + 2);
-            if (k == 1 || C == 0xffffffffu || cost < best) {
+            const float cost = time(lane_of(wave_scan(sum), 63) * c.kv_heads, largest(longest)) + 10.0f;
+            if (cost < best) {
                 best = cost;
                 C = Ck;
             }
         }
+        if (blockIdx.x == 0) *plan = C;
         if (c.n > 64) read(0);
     }
-    if (!JOIN && !slots && c.n <= 64) {
+    if (!JOIN && C == kWhole && c.n <= 64) {
         // No parts: the tiles with the most units first, whichever sequence they are of, so that the last
         // ones to start are short.  reach(U): tiles of the lane's sequence that have at least U units, which
         // are its last ones: the largest U that idx tiles or fewer reach is that of tile idx.
@@ -605,7 +624,7 @@ __device__ __forceinline__ bool find_item(const AttnCache &c, uint32_t group, ui
     for (uint32_t b0 = 0; b0 < c.n; b0 += 64) {
         if (b0) read(b0);
         uint32_t t = ((uint32_t)s.nq * group + BM - 1) / BM, parts = 1;
-        if (C != 0xffffffffu) parts = max(1u, ((uint32_t)(s.len + UNIT - 1) / UNIT + C - 1) / C);
+        if (C != kWhole) parts = max(1u, ((uint32_t)(s.len + UNIT - 1) / UNIT + C - 1) / C);
         const uint32_t all = t * parts * c.kv_heads, mine = JOIN ? t * c.kv_heads : all;
         const uint32_t end = wave_scan(mine), send = JOIN ? wave_scan(all) : 0;
         const uint64_t hit = __ballot(base + end > idx);
@@ -795,7 +814,7 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
     const uint32_t g = lane >> 4, col = lane & 15;
     Place pl;
     uint32_t left;
-    if (!find_place<G::BM, false>(A.c, A.group, slots, unit, blockIdx.x, &left, pl)) return;
+    if (!find_place<G::BM, false>(A.c, A.group, slots, unit, blockIdx.x, (uint32_t *)A.work, &left, pl)) return;
 
     // A tile of the share: its rows, and the wave's keys.
     struct Segment {
@@ -820,7 +839,7 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
         return sg;
     };
     // the tile after it; the next sequence has been read ahead
-    Seq ahead = sequence(A.c, min(pl.b + 1, A.c.n - 1));
+    Seq ahead;
     auto advance = [&](uint32_t took) {
         left -= took;
         if (!left) return false;
@@ -871,6 +890,7 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
     };
     Segment sg = segment();
     start(sg);
+    ahead = sequence(A.c, min(pl.b + 1, A.c.n - 1));
 
     // tile after tile until the share is used up; the next one's first loads go out before this one's end
     for (;;) {
@@ -1007,7 +1027,7 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
     for (int i = 0; i < NB; ++i) *(f32x4 *)(mine + ecol * D + ((i * 16 + eg * 4) ^ ((ecol & 7) << 2))) = o[i];
     __syncthreads();
     // a workgroup's share starts with at most one tile's end and ends with at most one tile's start
-    float *const part = (float *)A.work + (2 * (uint64_t)blockIdx.x + done.opens) * G::SLOT;
+    float *const part = (float *)A.work + kPlanFloats + (2 * (uint64_t)blockIdx.x + done.opens) * G::SLOT;
     const float vs = C == kE4M3 && A.c.v_scale ? A.c.v_scale[it.h] : 1.0f;
 #pragma unroll
     for (int e = 0; e < 16 * D / 4 / (64 * W); ++e) {
@@ -1057,7 +1077,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots, u
     uint32_t parts;
     uint64_t slot0, next;  // the first part's sums, and from the second's to the next
     if constexpr (UNIT > 0) {
-        if (!find_item<BM, UNIT, true>(A.c, A.group, slots, blockIdx.x / BLOCKS, it)) return;
+        if (!find_item<BM, UNIT, true>(A.c, A.group, slots, blockIdx.x / BLOCKS, (uint32_t *)A.work, it)) return;
         int32_t end;
         uint32_t per;
         tile_keys<BM, UNIT>(it, A.group, &end, &per, &parts);
@@ -1066,7 +1086,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots, u
     } else {
         Place p;
         uint32_t per;
-        if (!find_place<BM, true>(A.c, A.group, slots, unit, blockIdx.x / BLOCKS, &per, p)) return;
+        if (!find_place<BM, true>(A.c, A.group, slots, unit, blockIdx.x / BLOCKS, (uint32_t *)A.work, &per, p)) return;
         const uint32_t w = p.start / per;
         parts = (p.start + p.units - 1) / per - w + 1;
         slot0 = 2 * (uint64_t)w;
@@ -1075,7 +1095,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots, u
     }
     const uint32_t tr = it.rt * BM + rr;
     if (parts == 1 || it.rt * BM + rb >= (uint32_t)it.nq * A.group) return;
-    const float *const first = (const float *)A.work + slot0 * SLOT;
+    const float *const first = (const float *)A.work + kPlanFloats + slot0 * SLOT;
     const uint64_t step = next * SLOT;
     const uint32_t pg = threadIdx.x / LD % NG, dl = threadIdx.x % LD, d = (blockIdx.y * LD + dl) * 4;
     // a group keeps its own running maximum; the groups are joined like the parts
@@ -1124,42 +1144,46 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots, u
 }
 
 // ---- prompts ---------------------------------------------------------------------
-// A workgroup takes 128 rows of one key head, 32 per wave, and walks over tiles of
-// BK keys that its four waves share in LDS as bf16 planes: an E4M3 cache is widened
-// and an f32 one split once, as the tile is staged.
-template <uint32_t R, uint32_t C, int D>
+// A workgroup takes BM rows of one key head, 32 per wave, and walks over tiles of BK
+// keys that its four waves share in LDS as bf16 planes: an E4M3 cache is widened and
+// an f32 one split once, as the tile is staged.  KS = 1: 128 rows, each wave all keys
+// of a tile.  KS = 2: 64 rows, two waves share 32 rows and take half of a tile's keys
+// each: for few rows, and where 128-row tiles would leave CUs idle.
+template <uint32_t R, uint32_t C, int D, int KS>
 struct TileCfg {
-    static constexpr int QT = kTerms<R>, KT = kTerms<C>, BM = 128;
-    static constexpr int BK = KT == 3 || D == 256 || (QT == 3 && D == 128) ? 32 : 64;
+    static constexpr int QT = kTerms<R>, KT = kTerms<C>, BM = 128 / KS;
+    static constexpr int BK = KS == 1 && (KT == 3 || D == 256 || (QT == 3 && D == 128)) ? 32 : 64;
     static constexpr int PLANE = BK * D * 2, HALF = PLANE * KT;       // bytes of a tile's K, and of its V
     static constexpr int BUF = 4 * HALF <= 128 * 1024 ? 2 : 1;
+    static constexpr int OCC = 2 * BUF * HALF > 80 * 1024 || D == 256 ? 1 : 2;  // waves on a SIMD
     static constexpr int SLOT = BM * (D + 2);
+    static constexpr bool FITS = 2 * HALF <= 160 * 1024;
 };
 
-template <uint32_t R, uint32_t C, int D>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A, uint32_t slots) {
-    using G = TileCfg<R, C, D>;
-    constexpr int QT = G::QT, KT = G::KT, BK = G::BK, NS = D / 16, NB = D / 32, NN = BK / 32;
+template <uint32_t R, uint32_t C, int D, int KS>
+__global__ __launch_bounds__(256, (TileCfg<R, C, D, KS>::OCC)) void k_attn_tile(AttnArgs A, uint32_t slots) {
+    using G = TileCfg<R, C, D, KS>;
+    constexpr int QT = G::QT, KT = G::KT, BK = G::BK, WK = BK / KS, NS = D / 16, NB = D / 32, NN = WK / 32;
     constexpr int PN = Piece<C>::N, SUB = PN / 8, NL = BK * D / PN / 256;
     __shared__ __align__(16) uint8_t sh[G::BUF * 2 * G::HALF];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t g = lane >> 5, col = lane & 31;
+    const uint32_t g = lane >> 5, col = lane & 31, wrow = (KS == 1 ? wave : wave & 1) * 32, kq = KS == 1 ? 0 : wave >> 1;
     Item it;
-    if (!find_item<G::BM, BK, false>(A.c, A.group, slots, blockIdx.x, it)) return;
+    if (!find_item<G::BM, BK, false>(A.c, A.group, slots, blockIdx.x, (uint32_t *)A.work, it)) return;
     int32_t end;
     uint32_t per, parts;
     tile_keys<G::BM, BK>(it, A.group, &end, &per, &parts);
     if (it.part >= parts) return;
     const int32_t first = (int32_t)(it.part * per * BK), stop = min(end, first + (int32_t)(per * BK));
 
-    const uint32_t rows = (uint32_t)it.nq * A.group, r = it.rt * G::BM + wave * 32 + col;
+    const uint32_t rows = (uint32_t)it.nq * A.group, r = it.rt * G::BM + wrow + col;
     const bool valid = r < rows;
     const uint32_t tok = valid ? r / A.group : 0, x = it.h * A.group + (valid ? r - tok * A.group : 0);
     const uint64_t row = (uint64_t)(it.r0 + (int32_t)tok);
     const int32_t sees = valid ? min(max(it.len - it.nq + (int32_t)tok + 1, 0), end) : 0;
     const int32_t sees_min = __builtin_amdgcn_readfirstlane(sees);
     // the wave's last row; a wave without rows sees nothing
-    const uint32_t w0 = it.rt * G::BM + wave * 32, wl = min(w0 + 32, rows);
+    const uint32_t w0 = it.rt * G::BM + wrow, wl = min(w0 + 32, rows);
     const int32_t sees_max = w0 < rows ? min(max(it.len - it.nq + (int32_t)((wl - 1) / A.group) + 1, 0), end) : 0;
     float c2 = A.scale * (C == kE4M3 && A.c.k_scale ? A.c.k_scale[it.h] : 1.0f) * 1.44269504088896340736f;
     const uint32_t flip = c2 < 0.0f ? 0x80000000u : 0u;
@@ -1184,19 +1208,34 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
     Piece<C> kr[NL], vr[NL];
     const uint32_t ch = lane % (D / PN), tkey = wave * KW + lane / (D / PN), ts = (uint32_t)A.c.token_stride * kSize<C>;
     const uint32_t voff = (tkey & 15) * ts + ch * PN * kSize<C>;
-    auto load = [&] {
-        const uint64_t at = runs.place(A.c, head, 0, &bad_page) * kSize<C>;
+    uint64_t at_run;
+    auto load_keys = [&] {
+        at_run = runs.place(A.c, head, 0, &bad_page) * kSize<C>;
         runs.fetch(A.c);
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            kr[i].load((const uint8_t *)A.c.k + at + i * KL * ts + voff);
-            vr[i].load((const uint8_t *)A.c.v + at + i * KL * ts + voff);
-        }
+        for (int i = 0; i < NL; ++i) kr[i].load((const uint8_t *)A.c.k + at_run + i * KL * ts + voff);
+    };
+    auto load_values = [&] {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) vr[i].load((const uint8_t *)A.c.v + at_run + i * KL * ts + voff);
     };
     // masks cut through the workgroup's tiles from here on
     const int32_t cut = min(max(it.len - it.nq + (int32_t)(it.rt * G::BM / A.group) + 1, 0), end);
     bool bad = false;
-    auto store = [&](int32_t key0, uint8_t *to) {
+    auto put = [&](const Piece<C> &piece, int i, uint8_t *to) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            bf8 x[KT];
+            piece.terms(u, x);
+#pragma unroll
+            for (int t = 0; t < KT; ++t) *(bf8 *)(to + t * G::PLANE + lds_at<D>(i * KL + tkey, ch * SUB + u)) = x[t];
+        }
+    };
+    auto store_keys = [&](uint8_t *to) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) put(kr[i], i, to);
+    };
+    auto store_values = [&](int32_t key0, uint8_t *to) {
         if (key0 + BK > cut) {
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
@@ -1205,145 +1244,187 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_attn_tile(AttnArgs A,
             }
         }
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-#pragma unroll
-            for (int u = 0; u < SUB; ++u) {
-                bf8 k[KT], v[KT];
-                kr[i].terms(u, k);
-                vr[i].terms(u, v);
-                const uint32_t at = lds_at<D>(i * KL + tkey, ch * SUB + u);
-#pragma unroll
-                for (int t = 0; t < KT; ++t) {
-                    *(bf8 *)(to + t * G::PLANE + at) = k[t];
-                    *(bf8 *)(to + G::HALF + t * G::PLANE + at) = v[t];
-                }
-            }
-        }
+        for (int i = 0; i < NL; ++i) put(vr[i], i, to + G::HALF);
     };
+    const uint32_t klds0 = lds_at<D>(col, g);
+    const uint32_t vlds0 = lds_at<D>(g * 4 + ((lane & 15) >> 2), ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) + (lane & 1) * 8;
     uint32_t buf = 0;
     if (first < stop) {
-        load();
-        store(first, sh);
+        load_keys();
+        load_values();
+        store_keys(sh);
+        store_values(first, sh);
     }
     __syncthreads();
     for (int32_t key0 = first; key0 < stop; key0 += BK) {
         const bool more = key0 + BK < stop;
-        if (more) load();
-        const uint8_t *const ks = sh + buf * 2 * G::HALF, *const vs = ks + G::HALF;
-        if (key0 < sees_max) {
-            const bool masked = key0 + BK > sees_min;
-            const float cc = masked ? 1.0f : c2;
-            f32x16 sc[NN];
-            bf8 pt[BK / 16][QT];
-            float mu;
-            // scores of 32 keys
-            auto scores = [&](int n) {
+        uint8_t *const next = sh + (G::BUF == 2 ? (buf ^ 1) : 0) * 2 * G::HALF;
+        if (more) {
+            load_keys();
+            load_values();
+        }
+        const int32_t kw = key0 + (int32_t)kq * WK;  // the wave's keys
+        // where piece 0 of the lane's K and V reads is: piece n is at that ^ 16 n, worked out as it is needed
+        uint32_t klds = klds0, vlds = vlds0;
+        asm volatile("" : "+v"(klds), "+v"(vlds));
+        const uint8_t *const ks = sh + buf * 2 * G::HALF + kq * WK * D * 2, *const vs = ks + G::HALF;
+        const bool masked = kw + WK > sees_min;
+        const float cc = masked ? 1.0f : c2;
+        f32x16 sc[NN];
+        bf8 pt[WK / 16][QT];
+        float mu;
+        // scores of 32 keys
+        auto scores = [&](int n) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sc[n][e] = 0.0f;
+            for (int e = 0; e < 16; ++e) sc[n][e] = 0.0f;
 #pragma unroll
-                for (int s = 0; s < NS; ++s) {
-                    bf8 k[KT];
+            for (int s = 0; s < NS; ++s) {
+                bf8 k[KT];
 #pragma unroll
-                    for (int t = 0; t < KT; ++t) k[t] = *(const bf8 *)(ks + t * G::PLANE + lds_at<D>(n * 32 + col, s * 2 + g));
-                    sc[n] = product<KT, QT>(k, q[s], sc[n], mfma32);
+                for (int t = 0; t < KT; ++t) k[t] = *(const bf8 *)(ks + t * G::PLANE + n * 32 * D * 2 + (klds ^ s << 5));
+                sc[n] = product<KT, QT>(k, q[s], sc[n], mfma32);
+            }
+        };
+        // their mask and maximum; what was summed so far is scaled down where that rises
+        auto largest = [&](int n) {
+            if (masked)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    sc[n][e] = kw + n * 32 + (e / 4) * 8 + (int32_t)g * 4 + e % 4 < sees ? sc[n][e] * c2 : -INFINITY;
+            float m[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[e] = fmaxf(fmaxf(sc[n][e], sc[n][e + 4]), fmaxf(sc[n][e + 8], sc[n][e + 12]));
+            const float mx = across32(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))) * cc;
+            if (__any(mx > st.m + 8.0f)) {
+                const float mn = fmaxf(st.m, mx), f = exp2_hw(st.m - finite_max(mn));
+                st.l *= f;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) o[i] *= f;
+                st.m = mn;
+            }
+            mu = finite_max(st.m);
+        };
+        // weights of 16 keys
+        auto weights = [&](int n) {
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = exp2_hw(__builtin_fmaf(sc[n / 2][(n % 2) * 8 + i], cc, -mu));
+            st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            split8<QT>(p, pt[n]);
+        };
+        // their products with the values
+        auto values = [&](int n) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                bf8 v[KT];
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    const uint32_t at = t * G::PLANE + n * 16 * D * 2 + (vlds ^ i << 6);
+                    const u32x2 a = read_tr(vs, at), b = read_tr(vs, at + 8 * D * 2);
+                    v[t] = __builtin_bit_cast(bf8, u32x4{a[0], a[1], b[0], b[1]});
                 }
-            };
-            // their mask and maximum; what was summed so far is scaled down where that rises
-            auto largest = [&](int n) {
-                if (masked)
+                o[i] = product<KT, QT>(v, pt[n], o[i], mfma32);
+            }
+        };
+        if (kw < sees_max) {
+            if constexpr (QT == 3) {
+                // the registers are full of q's terms: one thing after the other
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        sc[n][e] = key0 + n * 32 + (e / 4) * 8 + (int32_t)g * 4 + e % 4 < sees ? sc[n][e] * c2 : -INFINITY;
-                float m[4];
+                for (int n = 0; n < NN; ++n) {
+                    scores(n);
+                    __builtin_amdgcn_sched_barrier(0);
+                    largest(n);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) m[e] = fmaxf(fmaxf(sc[n][e], sc[n][e + 4]), fmaxf(sc[n][e + 8], sc[n][e + 12]));
-                const float mx = across32(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))) * cc;
-                if (__any(mx > st.m + 8.0f)) {
-                    const float mn = fmaxf(st.m, mx), f = exp2_hw(st.m - finite_max(mn));
-                    st.l *= f;
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) o[i] *= f;
-                    st.m = mn;
-                }
-                mu = finite_max(st.m);
-            };
-            // weights of 16 keys
-            auto weights = [&](int n) {
-                float p[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) p[i] = exp2_hw(__builtin_fmaf(sc[n / 2][(n % 2) * 8 + i], cc, -mu));
-                st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-                split8<QT>(p, pt[n]);
-            };
-            // their products with the values
-            const uint32_t tk = g * 4 + ((lane & 15) >> 2), tc = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), tb = (lane & 1) * 8;
-            auto values = [&](int n) {
-#pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                    bf8 v[KT];
-#pragma unroll
-                    for (int t = 0; t < KT; ++t) {
-                        const uint32_t at = t * G::PLANE + lds_at<D>(tk, i * 4 + tc) + tb + n * 16 * D * 2;
-                        const u32x2 a = read_tr(vs, at), b = read_tr(vs, at + 8 * D * 2);
-                        v[t] = __builtin_bit_cast(bf8, u32x4{a[0], a[1], b[0], b[1]});
+                    for (int h = 2 * n; h < 2 * n + 2; ++h) {
+                        weights(h);
+                        __builtin_amdgcn_sched_barrier(0);
+                        values(h);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    o[i] = product<KT, QT>(v, pt[n], o[i], mfma32);
                 }
-            };
-            // Matrix instructions beside vector ones that do not need them: the second half's scores with the first
-            // half's weights, the first half's values with the second half's weights.
-            scores(0);
-            largest(0);
-            if constexpr (NN == 2) {
-                scores(1);
-                weights(0);
-                weights(1);
-                largest(1);
-                weights(2);
-                weights(3);
-                values(0);
-                values(1);
-                values(2);
-                values(3);
             } else {
+                // matrix instructions beside vector ones that do not need them: the second half's scores beside the
+                // first half's weights, the first half's values beside the second half's weights
+                scores(0);
+                largest(0);
+                if constexpr (NN == 2) scores(1);
                 weights(0);
                 weights(1);
-                values(0);
-                values(1);
+                if constexpr (NN == 2) {
+                    largest(1);
+                    weights(2);
+                    weights(3);
+                }
+#pragma unroll
+                for (int n = 0; n < 2 * NN; ++n) values(n);
             }
         }
         if (G::BUF == 1) __syncthreads();
-        if (more) store(key0 + BK, sh + (G::BUF == 2 ? (buf ^ 1) : 0) * 2 * G::HALF);
+        if (more) {
+            store_keys(next);
+            store_values(key0 + BK, next);
+        }
         if (G::BUF == 2) buf ^= 1;
         __syncthreads();
     }
 
     if (bad_page) flag(A.c.err, kAttnBadPage);
-    if (__syncthreads_or(bad))
-        add_not_finite<C, D, true>(A.c, it, max(first, cut / BK * BK), min(stop, it.len), sees, o);
+    const bool any_bad = __syncthreads_or(bad);
+    const uint32_t etid = thread_id(), ecol = etid & 31, eg = etid >> 5 & 1, elane = etid & 63;
     st.l += __shfl_xor(st.l, 32);
-    if (!valid) return;
-    const uint32_t rr = wave * 32 + col;
+    if constexpr (KS == 2) {
+        // the second two waves' sums to the first two
+        float *const to = (float *)sh + wrow / 32 * (32 * D + 64);
+        if (kq) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *(f32x4 *)(to + (i * 4 + e / 4) * 256 + elane * 4) = f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+            if (eg == 0) {
+                to[32 * D + ecol] = st.m;
+                to[32 * D + 32 + ecol] = st.l;
+            }
+        }
+        __syncthreads();
+        if (kq) return;
+        const float om = to[32 * D + ecol], m = fmaxf(st.m, om), f0 = exp2_hw(st.m - finite_max(m)), f1 = exp2_hw(om - finite_max(m));
+        st.l = __builtin_fmaf(to[32 * D + 32 + ecol], f1, st.l * f0);
+        st.m = m;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const f32x4 z = *(const f32x4 *)(to + (i * 4 + e / 4) * 256 + elane * 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[i][e + j] = __builtin_fmaf(z[j], f1, o[i][e + j] * f0);
+            }
+    }
+    if (any_bad) add_not_finite<C, D, true>(A.c, it, max(first, cut / BK * BK), min(stop, it.len), sees, o);
+    const uint32_t rr = wrow + ecol, er = it.rt * G::BM + rr;
+    if (er >= rows) return;
+    const uint32_t etok = er / A.group, ex = it.h * A.group + er - etok * A.group;
+    const uint64_t erow = (uint64_t)(it.r0 + (int32_t)etok);
     const float vsc = C == kE4M3 && A.c.v_scale ? A.c.v_scale[it.h] : 1.0f;
     if (parts > 1) {
-        float *const part = (float *)A.work + (uint64_t)it.slot * G::SLOT;
+        float *const part = (float *)A.work + kPlanFloats + (uint64_t)it.slot * G::SLOT;
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-                *(f32x4 *)(part + rr * D + i * 32 + e * 2 + g * 4) = f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
-        if (g == 0) {
+                *(f32x4 *)(part + rr * D + i * 32 + e * 2 + eg * 4) = f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+        if (eg == 0) {
             part[G::BM * D + rr] = st.m;
             part[G::BM * D + G::BM + rr] = st.l;
         }
         return;
     }
-    const float f = it.len - it.nq + (int32_t)tok + 1 > 0 ? vsc / st.l : 0.0f;
+    const float f = it.len - it.nq + (int32_t)etok + 1 > 0 ? vsc / st.l : 0.0f;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
-            write4<R>(A, row, x, D, i * 32 + e * 2 + g * 4, f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]}, f);
+            write4<R>(A, erow, ex, D, i * 32 + e * 2 + eg * 4, f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]}, f);
 }
 
 // The instance for a row type, cache type and head dimension.
@@ -1381,31 +1462,41 @@ void launch_append(const AppendArgs &A, uint32_t row_t, uint32_t dim, hipStream_
 
 namespace {
 
+enum Kernel { kSplit, kTile64, kTile128 };
+
 struct Plan {
-    bool tile;              // the prompt kernel
-    uint32_t tiles, slots;  // row tiles x key heads at most; workgroups that share them (0: one for each tile)
-    uint32_t unit;          // keys that go to one of them together
+    Kernel kernel;
+    uint32_t tiles, slots;  // row tiles x key heads at most; workgroups or parts that share them (0: one for each tile)
+    uint32_t unit;          // kSplit: keys that go to a workgroup together
 };
 
 Plan plan(const AttnArgs &A, uint32_t dim) {
     Plan p;
-    const uint64_t rows = (uint64_t)A.c.rows * A.group;
-    p.tile = A.c.row0 && rows > 64ull * A.c.n;
-    const uint32_t bm = p.tile ? 128 : 16;
+    const uint64_t rows = (uint64_t)A.c.rows * A.group, longest = (uint64_t)A.c.max_pages * A.c.page_size;
+    const bool f32 = A.c.dtype == kF32;
     // a sequence's last tile may be in part empty
-    p.tiles = (uint32_t)std::min<uint64_t>(rows / bm + A.c.n, rows) * A.c.kv_heads;
-    if (p.tile) {
-        p.slots = p.tiles < 512 ? 1024 : 0;  // two workgroups on a CU, in up to two rounds
+    auto tiles = [&](uint32_t bm) { return (uint32_t)std::min<uint64_t>(rows / bm + A.c.n, rows) * A.c.kv_heads; };
+    // Up to 16 rows a sequence the keys are read once by the kernel that streams them; 64-row tiles to 64 rows a
+    // sequence, and on short contexts while 128-row ones would not fill the CUs (no such instance for an f32 cache
+    // of 256: its tile does not fit the LDS).
+    const bool t64 = !(f32 && dim == 256);
+    p.kernel = rows <= 16ull * A.c.n ? kSplit
+               : t64 && (rows <= 64ull * A.c.n || (tiles(128) < 256 && longest <= 2048)) ? kTile64 : kTile128;
+    if (p.kernel != kSplit) {
+        // one or two workgroups on a CU (TileCfg::OCC), in up to two rounds; a few units are not worth joining
+        const uint32_t chip = dim == 256 || (f32 && (dim == 128 || p.kernel == kTile64)) ? 256 : 512;
+        p.tiles = tiles(p.kernel == kTile64 ? 64 : 128);
+        p.slots = p.tiles < chip && longest > 512 ? 2 * chip : 0;
         p.unit = 0;
         return p;
     }
     // as many workgroups as are on the chip at once, or tiles where those are more: shorter shares, which
     // the chip takes in turn; many tiles need no sharing
-    const bool f32 = A.c.dtype == kF32;
     const uint32_t chip = dim == 256 || (f32 && dim == 128) ? 256 : 512;
-    p.slots = p.tiles < 2048 ? std::max(chip, p.tiles) : 0;
+    p.tiles = tiles(16);
     p.unit = f32 && dim == 256 ? 64 : A.c.dtype == kE4M3 && dim <= 128 ? 256 : 128;  // SplitCfg::UNIT
-    while ((uint64_t)p.tiles * ((uint64_t)A.c.max_pages * A.c.page_size / p.unit + 2) > 0x7fffffffull) p.unit *= 2;
+    p.slots = p.tiles < 2048 && longest > p.unit ? std::max(chip, p.tiles) : 0;
+    while ((uint64_t)p.tiles * (longest / p.unit + 2) > 0x7fffffffull) p.unit *= 2;
     return p;
 }
 
@@ -1413,29 +1504,39 @@ Plan plan(const AttnArgs &A, uint32_t dim) {
 
 uint64_t attn_work_bytes(const AttnArgs &A, uint32_t dim) {
     const Plan p = plan(A, dim);
-    return std::max<uint64_t>(16, (uint64_t)p.slots * (p.tile ? 128 : 2 * 16) * (dim + 2) * 4);
+    const uint64_t rows = p.kernel == kSplit ? 2 * 16 : p.kernel == kTile64 ? 64 : 128;
+    return (kPlanFloats + p.slots * rows * (dim + 2)) * 4;
 }
 
 void launch_attn(const AttnArgs &A, uint32_t row_t, uint32_t dim, hipStream_t st) {
     const Plan p = plan(A, dim);
-    const uint32_t grid = p.tile ? std::max(p.tiles, p.slots) : p.slots ? p.slots : p.tiles;
-    // with many parts a tile, a workgroup joins 32 numbers of a row, else as many rows as its lanes hold
     auto join = [&](auto r, auto c, auto d, auto bm, auto unit) {
+        // with many parts a tile, a workgroup joins 32 numbers of a row or two rows, else as many rows as its lanes hold
         constexpr int all = 1024 / d() < bm() ? 1024 / d() : bm();
-        if (p.slots > 16 * p.tiles)
-            k_attn_join<r(), c(), d(), bm(), unit(), 8, 1><<<dim3(p.tiles * bm(), d() / 32), 256, 0, st>>>(A, p.slots, p.unit);
-        else if (p.slots)
+        if (!p.slots) return;
+        if (p.slots <= 16 * p.tiles)
             k_attn_join<r(), c(), d(), bm(), unit(), d() / 4, all><<<p.tiles * (bm() / all), 256, 0, st>>>(A, p.slots, p.unit);
+        else if constexpr (bm() == 16)
+            k_attn_join<r(), c(), d(), bm(), unit(), 8, 1><<<dim3(p.tiles * bm(), d() / 32), 256, 0, st>>>(A, p.slots, p.unit);
+        else
+            k_attn_join<r(), c(), d(), bm(), unit(), d() / 4, 2><<<p.tiles * (bm() / 2), 256, 0, st>>>(A, p.slots, p.unit);
     };
     pick(row_t, A.c.dtype, dim, [&](auto r, auto c, auto d) {
-        if (p.tile) {
-            using G = TileCfg<r(), c(), d()>;
-            k_attn_tile<r(), c(), d()><<<grid, 256, 0, st>>>(A, p.slots);
-            join(r, c, d, std::integral_constant<int, G::BM>{}, std::integral_constant<int, G::BK>{});
+        auto tile = [&](auto ks) {
+            using G = TileCfg<r(), c(), d(), ks()>;
+            if constexpr (G::FITS) {
+                k_attn_tile<r(), c(), d(), ks()><<<std::max(p.tiles, p.slots), 256, 0, st>>>(A, p.slots);
+                join(r, c, d, std::integral_constant<int, G::BM>{}, std::integral_constant<int, G::BK>{});
+            }
+        };
+        if (p.kernel == kTile128) {
+            tile(std::integral_constant<int, 1>{});
+        } else if (p.kernel == kTile64) {
+            tile(std::integral_constant<int, 2>{});
         } else {
             using G = SplitCfg<r(), c(), d()>;
-            k_attn_split<r(), c(), d()><<<grid, 64 * G::W, 0, st>>>(A, p.slots, p.unit);
-            join(r, c, d, std::integral_constant<int, G::BM>{}, std::integral_constant<int, 0>{});
+            k_attn_split<r(), c(), d()><<<p.slots ? p.slots : p.tiles, 64 * G::W, 0, st>>>(A, p.slots, p.unit);
+            join(r, c, d, std::integral_constant<int, 16>{}, std::integral_constant<int, 0>{});
         }
     });
 }
