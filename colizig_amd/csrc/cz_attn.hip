@@ -1343,20 +1343,21 @@ __global__ __launch_bounds__(256, (TileCfg<R, C, D, KS>::OCC)) void k_attn_tile(
                     }
                 }
             } else {
-                // matrix instructions beside vector ones that do not need them: the second half's scores beside the
-                // first half's weights, the first half's values beside the second half's weights
+                // the second half's scores (matrix) beside the first half's weights (vector)
                 scores(0);
                 largest(0);
                 if constexpr (NN == 2) scores(1);
                 weights(0);
                 weights(1);
+                values(0);
+                values(1);
                 if constexpr (NN == 2) {
-                    largest(1);
+                    largest(1);  // (what it scales down has to hold the first half)
                     weights(2);
                     weights(3);
+                    values(2);
+                    values(3);
                 }
-#pragma unroll
-                for (int n = 0; n < 2 * NN; ++n) values(n);
             }
         }
         if (G::BUF == 1) __syncthreads();

@@ -211,6 +211,26 @@ def test_prompt_draft(dev, rows, cache):
     p.check(p.attend(dev))
 
 
+@pytest.mark.parametrize("rows,cache", TYPES)
+@pytest.mark.parametrize("heads,new,past", [
+    ((8, 2, 128), [1], [3000]), ((8, 2, 128), [7, 1], [2500, 300]), ((8, 2, 128), [150], [0]), ((8, 2, 128), [200], [2200]),
+    ((4, 4, 64), [300], [2100]), ((4, 2, 256), [140], [2100]), ((16, 2, 64), [60], [100]),
+])
+def test_rising_scores(dev, rows, cache, heads, new, past):
+    """Scores that spread over many powers of e and grow with the position, so
+    that a row's largest rises again and again: every kernel and tile size (one
+    token, few rows, 64- and 128-row tiles, parts) scales down what it holds."""
+    say("rising scores", rows, cache, heads, new, past)
+    p = H.Problem(rows, cache, heads, new, [a + b for a, b in zip(new, past)], 32, q_scale=3.0, seed=28)
+    for b in range(p.n):
+        k = H.decode(p.get(p.k, b, p.len[b]), cache)
+        k *= (0.2 + 2.0 * np.arange(p.len[b]) / p.len[b])[:, None, None]
+        p.set(p.k, b, 0, H.encode(k, cache))
+    total = p.row0[-1]
+    sel = None if total < 40 else set(np.random.default_rng(1).integers(0, total, 40)) | {0, total - 1}
+    p.check(p.attend(dev, decode_form=max(new) == 1 and len(new) == 1), rows=sel)
+
+
 def test_prompt_rows_before_the_start(dev):
     """More rows than tokens: rows at negative positions see nothing and give zeros."""
     say("prompt: rows without a key")
@@ -219,6 +239,14 @@ def test_prompt_rows_before_the_start(dev):
     got = p.attend(dev)
     assert not got[:2, :4 * 64].any()
     p.check(got)
+    # whole tiles of them, in each tile size
+    for cache in ("bf16", "f32"):
+        for heads, n in (((4, 1, 64), 300), ((32, 2, 256), 700)):
+            p = H.Problem("f32", cache, heads, [n, 2], [n, 2], seed=29)
+            p.len[0] = 20
+            got = p.attend(dev)
+            assert not got[:n - 20, :heads[0] * heads[2]].any()
+            p.check(got, rows=set(range(n - 25, n + 2)))
 
 
 @pytest.mark.parametrize("rows,cache", TYPES)
