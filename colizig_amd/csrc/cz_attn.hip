@@ -63,13 +63,19 @@ constexpr int kTerms = T == kF32 ? 3 : 1;
 template <uint32_t T>
 constexpr int kSize = T == kF32 ? 4 : T == kBF16 ? 2 : 1;
 
-// x in N terms: one rounds to nearest.  Infinities have no lower terms (inf - inf);
+// x in N terms: one or two round to nearest (8 and 16 bits).  In three, infinities have no lower terms (inf - inf);
 // a NaN stays one in some term.
 template <int N>
 __device__ __forceinline__ void split8(const float (&x)[8], bf8 (&t)[N]) {
     if constexpr (N == 1) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) t[0][i] = (__bf16)x[i];
+    } else if constexpr (N == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            t[0][i] = (__bf16)x[i];
+            t[1][i] = (__bf16)(x[i] - (float)t[0][i]);
+        }
     } else {
         float r[8];
 #pragma unroll
@@ -790,6 +796,7 @@ __device__ __forceinline__ void add_not_finite(const AttnCache &c, const Item &i
 template <uint32_t R, uint32_t C, int D>
 struct SplitCfg {
     static constexpr int QT = kTerms<R>, KT = kTerms<C>, BM = 16;
+    static constexpr int PT = QT == 1 ? 2 : 3;  // of the weights: the matrix cores have time to spare here
     static constexpr int KEYS = C == kE4M3 && D <= 128 ? 64 : 32;  // about 8 KB of keys and of values in flight a wave
     static constexpr int W = KT == 3 && D == 256 ? 2 : 4, UNIT = W * KEYS;  // waves: as many as their tiles fit the LDS
     static constexpr int OCC = D == 256 ? 1 : KT == 3 ? (D == 64 ? 2 : 1) : D == 64 ? 3 : 2;  // waves on a SIMD
@@ -806,7 +813,7 @@ template <uint32_t R, uint32_t C, int D>
 __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OCC)) void k_attn_split(AttnArgs A, uint32_t slots,
                                                                                                  uint32_t unit) {
     using G = SplitCfg<R, C, D>;
-    constexpr int QT = G::QT, KT = G::KT, W = G::W, NS = D / 32, NB = D / 16, KEYS = G::KEYS, NR = KEYS / 16;
+    constexpr int QT = G::QT, KT = G::KT, PT = G::PT, W = G::W, NS = D / 32, NB = D / 16, KEYS = G::KEYS, NR = KEYS / 16;
     constexpr int PN = Piece<C>::N, SUB = PN / 8, NK = NS / SUB, NV = KEYS * D / PN / 64;
     __shared__ __align__(16) uint8_t sh[W * G::WAVE];
     __shared__ float sh_m[W][16], sh_l[W][16];
@@ -988,8 +995,8 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
                 p[i] = exp2_hw(__builtin_fmaf(sc[n + i / 4][i % 4], cc, -mu));
                 st.l += p[i];
             }
-            bf8 pt[QT];
-            split8<QT>(p, pt);
+            bf8 pt[PT];
+            split8<PT>(p, pt);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
@@ -1000,7 +1007,7 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
                     const u32x2 a = read_tr(lds, at), b = read_tr(lds, at + 16 * D * 2);
                     v[t] = __builtin_bit_cast(bf8, u32x4{a[0], a[1], b[0], b[1]});
                 }
-                o[i] = product<KT, QT>(v, pt, o[i], mfma16);
+                o[i] = product<KT, PT>(v, pt, o[i], mfma16);
             }
         }
         __builtin_amdgcn_wave_barrier();
