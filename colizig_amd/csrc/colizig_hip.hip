@@ -1870,7 +1870,7 @@ bool attn_sizes_ok(const colizig_kv_cache *c, const colizig_attn_batch *b, int d
     if (!b->row0 && b->rows != b->n) return attn_no("without row0 there is one row per sequence");
     if (b->n > 0xffffffu || (uint64_t)b->rows * (q_heads + 2 * c->kv_heads) > 0x7fffffffu)
         return attn_no("too many sequences or rows for one call");
-    if ((uint64_t)b->max_pages * c->page_size > 0x7fffffffu) return attn_no("max_pages * page_size over 2^31 - 1");
+    if ((uint64_t)b->max_pages * c->page_size > (1u << 30)) return attn_no("max_pages * page_size over 2^30");
     return true;
 }
 

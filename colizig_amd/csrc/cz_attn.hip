@@ -430,6 +430,12 @@ __device__ __forceinline__ uint32_t lds_at(uint32_t key, uint32_t chunk) {
     return key * (D * 2) + ((chunk ^ f) << 4);
 }
 
+// A sequence that is the same for the whole wave, in scalar registers.
+__device__ __forceinline__ Seq uniform(const Seq &s) {
+    return Seq{__builtin_amdgcn_readfirstlane(s.r0), __builtin_amdgcn_readfirstlane(s.nq),
+               __builtin_amdgcn_readfirstlane(s.len)};
+}
+
 // Sums over the lanes up to each one.
 template <typename T>
 __device__ __forceinline__ T wave_scan(T x) {
@@ -480,6 +486,19 @@ template <int BM, bool JOIN>
 __device__ __forceinline__ bool find_place(const AttnCache &c, uint32_t group, uint32_t slots, uint32_t unit, uint32_t idx,
                                            uint32_t *plan, uint32_t *per, Place &p) {
     const uint32_t lane = threadIdx.x & 63;
+    if (!JOIN && !slots && !c.row0) {  // a row and so many tiles for each sequence: nothing to search
+        const uint32_t t = (group + BM - 1) / BM, each = t * c.kv_heads;
+        p.b = idx / each;
+        if (p.b >= c.n) return false;
+        p.s = uniform(sequence(c, p.b));
+        p.tiles = t;
+        p.units = 1;
+        p.unit0 = 0;
+        p.j = (idx - p.b * each) / c.kv_heads;
+        p.h = idx - p.b * each - p.j * c.kv_heads;
+        *per = 1;
+        return true;
+    }
     Seq s{0, 0, 0};  // of the lane's sequence; up to 64 are read once
     auto read = [&](uint32_t b0) {
         s = Seq{0, 0, 0};
@@ -535,6 +554,22 @@ template <int BM, int UNIT, bool JOIN>
 __device__ __forceinline__ bool find_item(const AttnCache &c, uint32_t group, uint32_t slots, uint32_t idx, uint32_t *plan,
                                           Item &it) {
     const uint32_t lane = threadIdx.x & 63;
+    if (!JOIN && !slots && !c.row0) {  // a row and so many tiles for each sequence: nothing to search
+        const uint32_t t = (group + BM - 1) / BM, each = t * c.kv_heads;
+        it.b = idx / each;
+        if (it.b >= c.n) return false;
+        const Seq q = uniform(sequence(c, it.b));
+        const uint32_t j = (idx - it.b * each) / c.kv_heads;
+        it.rt = t - 1 - j;
+        it.part = 0;
+        it.h = idx - it.b * each - j * c.kv_heads;
+        it.parts = 1;
+        it.slot = idx;
+        it.r0 = q.r0;
+        it.nq = q.nq;
+        it.len = q.len;
+        return true;
+    }
     Seq s{0, 0, 0};  // of the lane's sequence; up to 64 are read once
     auto read = [&](uint32_t b0) {
         s = Seq{0, 0, 0};
@@ -857,8 +892,7 @@ __global__ __launch_bounds__((64 * SplitCfg<R, C, D>::W), (SplitCfg<R, C, D>::OC
         pl.j = 0;
         do {
             if (++pl.b == A.c.n) return false;
-            pl.s = Seq{__builtin_amdgcn_readfirstlane(ahead.r0), __builtin_amdgcn_readfirstlane(ahead.nq),
-                       __builtin_amdgcn_readfirstlane(ahead.len)};
+            pl.s = uniform(ahead);
             pl.tiles = tiles_of<G::BM>(pl.s, A.group);
             ahead = sequence(A.c, min(pl.b + 1, A.c.n - 1));
         } while (!pl.tiles);
@@ -1090,6 +1124,8 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots, u
         tile_keys<BM, UNIT>(it, A.group, &end, &per, &parts);
         slot0 = it.slot;
         next = A.c.kv_heads;
+        // (rows that overlap, which has been flagged, can place a tile where no part is)
+        if (slot0 + (parts - 1) * next >= slots) return;
     } else {
         Place p;
         uint32_t per;
@@ -1098,6 +1134,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots, u
         parts = (p.start + p.units - 1) / per - w + 1;
         slot0 = 2 * (uint64_t)w;
         next = 2;
+        if (slot0 + 2 * (uint64_t)parts > 2 * (uint64_t)slots) return;
         it = Item{p.b, p.tiles - 1 - p.j, p.h, 0, 0, 0, p.s.r0, p.s.nq, p.s.len};
     }
     const uint32_t tr = it.rt * BM + rr;
@@ -1381,6 +1418,7 @@ __global__ __launch_bounds__(256, (TileCfg<R, C, D, KS>::OCC)) void k_attn_tile(
     const uint32_t etid = thread_id(), ecol = etid & 31, eg = etid >> 5 & 1, elane = etid & 63;
     st.l += __shfl_xor(st.l, 32);
     if constexpr (KS == 2) {
+        static_assert(2 * (32 * D + 64) * 4 <= G::BUF * 2 * G::HALF, "the sums fit the tiles' place");
         // the second two waves' sums to the first two
         float *const to = (float *)sh + wrow / 32 * (32 * D + 64);
         if (kq) {
@@ -1504,7 +1542,8 @@ Plan plan(const AttnArgs &A, uint32_t dim) {
     p.tiles = tiles(16);
     p.unit = f32 && dim == 256 ? 64 : A.c.dtype == kE4M3 && dim <= 128 ? 256 : 128;  // SplitCfg::UNIT
     p.slots = p.tiles < 2048 && longest > p.unit ? std::max(chip, p.tiles) : 0;
-    while ((uint64_t)p.tiles * (longest / p.unit + 2) > 0x7fffffffull) p.unit *= 2;
+    // (all units are counted in 32 bits)
+    while (p.slots && (uint64_t)p.tiles * (longest / p.unit + 2) > 0x7fffffffull) p.unit *= 2;
     return p;
 }
 

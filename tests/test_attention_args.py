@@ -64,7 +64,7 @@ def test_sizes_and_types(kw, why):
 
 @pytest.mark.parametrize("b,why", [
     (dict(n=0, rows=0), "at least 1"), (dict(rows=4), "one row per sequence"), (dict(max_pages=0), "at least 1"),
-    (dict(max_pages=1 << 30), "2^31"), (dict(n=1 << 28, rows=1 << 28), "too many"),
+    (dict(max_pages=(1 << 26) + 1), "2^30"), (dict(n=1 << 28, rows=1 << 28), "too many"),
 ])
 def test_batches(b, why):
     for call in (attend, append):

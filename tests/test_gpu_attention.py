@@ -424,6 +424,39 @@ def test_bad_pages_and_lengths_are_reported(dev):
     assert np.array_equal(p.dk.download(np.empty_like(p.k)), p.k)
 
 
+def test_rows_that_overlap_are_reported(dev):
+    """row0 that falls: cut to what is there, reported, nothing out of bounds (the rows' results are invalid)."""
+    say("falling row0")
+    hip = _lib.hip()
+    for new, lens in (([3] * 9, [500] * 9), ([40] * 9, [900] * 9), ([300] * 6, [3000] * 6)):
+        p = H.Problem("f32", "bf16", (8, 2, 64), new, lens, 64, seed=43)
+        p.attend(dev, launch=False)
+        total = int(p.row0[-1])
+        p.drow0.upload(np.array([0 if b % 2 == 0 else total for b in range(p.n + 1)], np.int32))
+        p.call()
+        assert hip.colizig_hip_sync() == -5 and "rows" in _lib.last_error()
+        dk, dv = dev.put(p.kx), dev.put(p.vx)
+        attn.append(p.cache, p.batch, "f32", p.dq.ptr, dk.ptr, dv.ptr, p.dout.ptr, p.hq)
+        assert hip.colizig_hip_sync() in (0, -5)
+        p.upload(dev)
+        p.call()
+        assert hip.colizig_hip_sync() in (0, -5)
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 64), (40, 1, 64)])
+def test_thousands_of_sequences(dev, heads):
+    """More sequences than workgroups, each a workgroup's own: no search for its place."""
+    say("5,000 sequences", heads)
+    rng = np.random.default_rng(4)
+    n = 5000
+    p = H.Problem("f32", "bf16", heads, [1] * n, list(rng.integers(0, 40, n)), seed=14)
+    sel = set(rng.integers(0, n, 200)) | {0, n - 1}
+    p.check(p.attend(dev, decode_form=True), rows=sel)
+    new = list(rng.integers(0, 4, 600))
+    p = H.Problem("bf16", "e4m3", heads, new, [a + int(b) for a, b in zip(new, rng.integers(0, 90, 600))], seed=15)
+    p.check(p.attend(dev))
+
+
 # ---- all of it together ---------------------------------------------------------------
 def test_projections_append_prompt_decode(dev, oracle_lib):
     """A layer's attention as a program runs it: FP8 q, k and v projections,
