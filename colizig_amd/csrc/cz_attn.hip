@@ -267,8 +267,14 @@ __device__ __forceinline__ void floats8(const float *p, float (&x)[8]) {
 // pieces.  A norm's sum goes over the group's lanes; a rotation's other half is
 // dims / 16 lanes away.  A workgroup takes TB rows: the three lookups one after the
 // other (sequence, length, page and angles) cost it some microseconds whatever it
-// moves, and a group's angles and weights serve all its vectors of the row.
-// Few rows are spread over blockIdx.y too.
+// moves, and a group's angles and weights serve all its vectors of the row.  Below
+// kAppendBlockRows rows a workgroup takes one pass over one row, and a row is spread
+// over blockIdx.y.
+//
+// Bound: HBM for prompts, those look-ups for few rows.  14,588 BF16 rows of 32 + 2 x 4
+// heads of 128 (301 MB) 69 us, 4.4 TB/s, where a large copy moves 5.2; one row 3.5 us.
+// Eight rows a workgroup 76 us; a workgroup a row with its passes one after the other
+// 164 us.
 template <uint32_t R, uint32_t C, int D, int TB>
 __global__ __launch_bounds__(256) void k_append(AppendArgs A) {
     constexpr uint32_t LV = D / 8, GROUPS = 256 / LV, STEP = GROUPS / TB, UNROLL = TB == 1 ? 1 : 4;
@@ -393,6 +399,12 @@ __global__ __launch_bounds__(256) void k_append(AppendArgs A) {
 // layout once its keys are counted in that order, so weights go from one matrix
 // instruction to the next in registers; V's side of it, 4 keys of one number, is
 // what the transposing LDS read gives.
+//
+// f32 accuracy on the bf16 matrix cores: an f32 is the sum of three bf16 numbers, so
+// q and the weights of f32 rows are three terms each and every product is exact (an
+// f32 cache's keys and values are three terms too, and of the nine products of two
+// numbers the six above 2^-24 are taken); sums are f32.  Nearer to 64 bits than f32
+// products and sums are: 3.6e-7 for 6.2e-7 over packed prompts.
 // 8 query numbers as terms, negated where `flip` is the sign bit.
 template <uint32_t R>
 __device__ __forceinline__ void query8(const void *q, uint64_t at, uint32_t flip, bf8 (&t)[kTerms<R>]) {
@@ -827,7 +839,16 @@ __device__ __forceinline__ void add_not_finite(const AttnCache &c, const Item &i
 // the keys each, KEYS at a time, loading keys straight into matrix operand
 // registers and values through their own LDS tiles.  The order of the head
 // dimension in the first product is free: lane group g holds numbers N g .. of each
-// 4 N, as one load brings them.
+// 4 N, as one load brings them.  No barrier but at a tile's end: a wave's LDS tile
+// is its own.
+//
+// Bound: HBM.  32 sequences of up to 16,001 tokens, BF16 cache of 4 heads of 128 (485
+// MB): 79 us, 6.2 TB/s, the rate of a plain read here; one of 131,071 tokens 46 us
+// (5.8 TB/s); 128 sequences on an E4M3 cache (594 MB) 122 us (4.9 TB/s: f32 rows'
+// three terms of half the bytes, and two tile ends a workgroup).  577 tokens take 9
+// us, five look-ups and loads one after the other.  With a part of each sequence a
+// workgroup instead of equal shares 95, 64 and 127 us; the next tile's loads after
+// this one's end 87 us for the first; three waves a SIMD the same time as two.
 template <uint32_t R, uint32_t C, int D>
 struct SplitCfg {
     static constexpr int QT = kTerms<R>, KT = kTerms<C>, BM = 16;
@@ -1192,7 +1213,22 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots, u
 // keys that its four waves share in LDS as bf16 planes: an E4M3 cache is widened and
 // an f32 one split once, as the tile is staged.  KS = 1: 128 rows, each wave all keys
 // of a tile.  KS = 2: 64 rows, two waves share 32 rows and take half of a tile's keys
-// each: for few rows, and where 128-row tiles would leave CUs idle.
+// each: for few rows, and where 128-row tiles would leave CUs idle (6 tokens on each
+// of 16 caches of 8,000, BF16: 52 us, 160 with 16-row tiles).
+//
+// Bound: the matrix cores and, at two waves a SIMD, the vector work of the softmax
+// beside them (39 and 37% of a SIMD's cycles at 8,192 BF16 tokens; the clock falls
+// under such load as it does under a large product).  8,192 tokens, 32 heads on 4 of
+// 128: 605 us, 910 TFLOP/s of the visible products, where a large bf16 product reaches
+// 1,220; packed prompts of f32 rows 340 us, 349 TFLOP/s and three times that in
+// products; 777 tokens on 20,000 cached in E4M3 305 us, 850 TFLOP/s.
+//
+// 64-key tiles but where registers or LDS are short: with three terms of q a 64-key
+// tile spills (444 us for 358).  A wave looks up one page a tile: four look-ups a wave
+// were as many scalar instructions as vector ones, 6% of the time.  Measured and not
+// kept: fixed interleaving of matrix and vector instructions (750 for 700 us), raised
+// priority of the waves in the first product (within 2%), values loaded only after the
+// keys are staged (spills).
 template <uint32_t R, uint32_t C, int D, int KS>
 struct TileCfg {
     static constexpr int QT = kTerms<R>, KT = kTerms<C>, BM = 128 / KS;

@@ -185,8 +185,8 @@ int colizig_hip_attn_append(const colizig_kv_cache *cache, const colizig_attn_ba
  *   out[b][x] = sum_j softmax_j(scale * q[b][x] . k_j) v_j,  j < len[b],
  * with the keys and values of head x / (q_heads / kv_heads).  A sequence of
  * length 0 gives zeros.  Products and sums of f32 rows are at f32 accuracy;
- * for BF16 rows the softmax weights are rounded to BF16 for their products,
- * and the result once.  out may be q.  work: device scratch of
+ * for BF16 rows the softmax weights are rounded to 16 bits, or to BF16 (more
+ * than 16 query heads a key head), for their products, and the result once.  out may be q.  work: device scratch of
  * colizig_hip_attn_work_bytes, 16-byte aligned, held by no other call that
  * may run at the same time (a captured graph's stays its own); its contents
  * mean nothing between calls.  A row's bits depend on how the lengths of the
@@ -199,7 +199,9 @@ int colizig_hip_attn_decode(const colizig_kv_cache *cache, const colizig_attn_ba
 /* The same for sequences of any number of new tokens (batch->row0 given): a
  * whole prompt (len = its tokens), a chunk of one or a draft on top of cached
  * tokens, several of them packed.  The keys and values of the new tokens are
- * in the cache already.  Arguments and results as for one token. */
+ * in the cache already.  Arguments and results as for one token; the softmax
+ * weights of BF16 rows are rounded to BF16 for their products, to 16 bits
+ * where there are 16 rows x query heads per key head and sequence or fewer. */
 int colizig_hip_attn_prompt(const colizig_kv_cache *cache, const colizig_attn_batch *batch, int dtype, const void *q,
                             uint64_t q_stride, void *out, uint64_t out_stride, uint32_t q_heads, float scale,
                             void *work, uint64_t work_bytes, void *stream);
