@@ -1235,9 +1235,13 @@ struct TileCfg {
     static constexpr int BK = KS == 1 && (KT == 3 || D == 256 || (QT == 3 && D == 128)) ? 32 : 64;
     static constexpr int PLANE = BK * D * 2, HALF = PLANE * KT;       // bytes of a tile's K, and of its V
     static constexpr int BUF = 4 * HALF <= 128 * 1024 ? 2 : 1;
-    static constexpr int OCC = 2 * BUF * HALF > 80 * 1024 || D == 256 ? 1 : 2;  // waves on a SIMD
+    // Three terms of a q of 256 do not fit the registers: the third waits in the LDS, in the order its
+    // reads take it.
+    static constexpr bool QLDS = QT == 3 && D == 256;
+    static constexpr int QBYTES = QLDS ? BM * D * 2 : 0, LDS = BUF * 2 * HALF + QBYTES;
+    static constexpr int OCC = LDS > 80 * 1024 || D == 256 ? 1 : 2;  // waves on a SIMD
     static constexpr int SLOT = BM * (D + 2);
-    static constexpr bool FITS = 2 * HALF <= 160 * 1024;
+    static constexpr bool FITS = LDS <= 160 * 1024;
 };
 
 template <uint32_t R, uint32_t C, int D, int KS>
@@ -1245,7 +1249,7 @@ __global__ __launch_bounds__(256, (TileCfg<R, C, D, KS>::OCC)) void k_attn_tile(
     using G = TileCfg<R, C, D, KS>;
     constexpr int QT = G::QT, KT = G::KT, BK = G::BK, WK = BK / KS, NS = D / 16, NB = D / 32, NN = WK / 32;
     constexpr int PN = Piece<C>::N, SUB = PN / 8, NL = BK * D / PN / 256;
-    __shared__ __align__(16) uint8_t sh[G::BUF * 2 * G::HALF];
+    __shared__ __align__(16) uint8_t sh[G::LDS];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t g = lane >> 5, col = lane & 31, wrow = (KS == 1 ? wave : wave & 1) * 32, kq = KS == 1 ? 0 : wave >> 1;
     Item it;
@@ -1269,9 +1273,17 @@ __global__ __launch_bounds__(256, (TileCfg<R, C, D, KS>::OCC)) void k_attn_tile(
     const uint32_t flip = c2 < 0.0f ? 0x80000000u : 0u;
     c2 = fabsf(c2);
 
-    bf8 q[NS][QT];
+    constexpr int QR = G::QLDS ? 2 : QT;  // terms of q in registers
+    bf8 q[NS][QR];
+    const uint32_t qlds = G::BUF * 2 * G::HALF + (wrow / 32 * NS * 64 + lane) * 16;
 #pragma unroll
-    for (int s = 0; s < NS; ++s) query8<R>(A.q, row * A.q_stride + (uint64_t)x * D + s * 16 + g * 8, flip, q[s]);
+    for (int s = 0; s < NS; ++s) {
+        bf8 all[QT];
+        query8<R>(A.q, row * A.q_stride + (uint64_t)x * D + s * 16 + g * 8, flip, all);
+#pragma unroll
+        for (int n = 0; n < QR; ++n) q[s][n] = all[n];
+        if constexpr (G::QLDS) *(bf8 *)(sh + qlds + s * 1024) = all[2];  // (waves of the same rows write the same)
+    }
     f32x16 o[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
@@ -1362,7 +1374,11 @@ __global__ __launch_bounds__(256, (TileCfg<R, C, D, KS>::OCC)) void k_attn_tile(
                 bf8 k[KT];
 #pragma unroll
                 for (int t = 0; t < KT; ++t) k[t] = *(const bf8 *)(ks + t * G::PLANE + n * 32 * D * 2 + (klds ^ s << 5));
-                sc[n] = product<KT, QT>(k, q[s], sc[n], mfma32);
+                bf8 all[QT];
+#pragma unroll
+                for (int w = 0; w < QR; ++w) all[w] = q[s][w];
+                if constexpr (G::QLDS) all[2] = *(const bf8 *)(sh + qlds + s * 1024);
+                sc[n] = product<KT, QT>(k, all, sc[n], mfma32);
             }
         };
         // their mask and maximum; what was summed so far is scaled down where that rises
@@ -1450,11 +1466,17 @@ __global__ __launch_bounds__(256, (TileCfg<R, C, D, KS>::OCC)) void k_attn_tile(
     }
 
     if (bad_page) flag(A.c.err, kAttnBadPage);
-    const bool any_bad = __syncthreads_or(bad);
+    // whether any thread staged a value that is not finite (the tiles' place is free)
+    if (lane == 0) ((uint32_t *)sh)[wave] = 0;
+    if (bad) ((uint32_t *)sh)[wave] = 1;
+    __syncthreads();
+    const u32x4 bads = *(const u32x4 *)sh;
+    const bool any_bad = bads[0] | bads[1] | bads[2] | bads[3];
+    if constexpr (KS == 2) __syncthreads();
     const uint32_t etid = thread_id(), ecol = etid & 31, eg = etid >> 5 & 1, elane = etid & 63;
     st.l += __shfl_xor(st.l, 32);
     if constexpr (KS == 2) {
-        static_assert(2 * (32 * D + 64) * 4 <= G::BUF * 2 * G::HALF, "the sums fit the tiles' place");
+        static_assert(2 * (32 * D + 64) * 4 <= G::LDS, "the sums fit the tiles' place");
         // the second two waves' sums to the first two
         float *const to = (float *)sh + wrow / 32 * (32 * D + 64);
         if (kq) {
