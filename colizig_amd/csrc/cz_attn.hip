@@ -612,7 +612,7 @@ __device__ __forceinline__ bool find_item(const AttnCache &c, uint32_t group, ui
         // Whole tiles, or parts for one round of the chip, or for two, by units of time: a start and an end cost
         // about two, joining ten, and beyond one round the work is spread evenly but for half a part.  196 tiles of
         // 325 units make 392 parts of 163 in one round, which leaves a quarter of the chip idle, or 980 of 65 in two
-        // (398 and 361 us); 500 of up to 32 units are best left whole (62 us for 82 in parts).
+        // (398 and 361 us when the rule was made); 500 of up to 32 units are best left whole (62 us for 82).
         const float chip = (float)(slots / 2);
         seen = lane_of(wave_scan(seen), 63) * (float)c.kv_heads / chip;
         auto time = [&](uint32_t items, uint32_t longest) {
@@ -846,9 +846,10 @@ __device__ __forceinline__ void add_not_finite(const AttnCache &c, const Item &i
 // MB): 79 us, 6.2 TB/s, the rate of a plain read here; one of 131,071 tokens 46 us
 // (5.8 TB/s); 128 sequences on an E4M3 cache (594 MB) 122 us (4.9 TB/s: f32 rows'
 // three terms of half the bytes, and two tile ends a workgroup).  577 tokens take 9
-// us, five look-ups and loads one after the other.  With a part of each sequence a
-// workgroup instead of equal shares 95, 64 and 127 us; the next tile's loads after
-// this one's end 87 us for the first; three waves a SIMD the same time as two.
+// us: 2.7 to find the place, 1.6 to the first loads, 3.7 to the end of the only step,
+// 0.8 to the end.  With a part of each sequence a workgroup instead of equal shares 95
+// us for the first; the next tile's loads after this one's end 87; three waves a SIMD
+// the same time as two.
 template <uint32_t R, uint32_t C, int D>
 struct SplitCfg {
     static constexpr int QT = kTerms<R>, KT = kTerms<C>, BM = 16;
@@ -1217,18 +1218,22 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots, u
 // of 16 caches of 8,000, BF16: 52 us, 160 with 16-row tiles).
 //
 // Bound: the matrix cores and, at two waves a SIMD, the vector work of the softmax
-// beside them (39 and 37% of a SIMD's cycles at 8,192 BF16 tokens; the clock falls
-// under such load as it does under a large product).  8,192 tokens, 32 heads on 4 of
-// 128: 605 us, 910 TFLOP/s of the visible products, where a large bf16 product reaches
-// 1,220; packed prompts of f32 rows 340 us, 349 TFLOP/s and three times that in
-// products; 777 tokens on 20,000 cached in E4M3 305 us, 850 TFLOP/s.
+// beside them (44 and 57% of a SIMD's cycles at 8,192 BF16 tokens, 53 and 57 with f32
+// rows; the clock falls under such load as it does under a large product).  8,192
+// tokens, 32 heads on 4 of 128: 605-618 us, 890-910 TFLOP/s of the visible products,
+// where a large bf16 product reaches 1,220; packed prompts of f32 rows 339-345 us, 345
+// TFLOP/s and three times that in products; 777 tokens on 20,000 cached in E4M3 305 us,
+// 850 TFLOP/s.  A short prompt (500 tokens of f32 rows, 28 us) is 4 us to find its
+// tile, 8 to the end of the first 64 keys and 2 to 4 for each 64 after.
 //
 // 64-key tiles but where registers or LDS are short: with three terms of q a 64-key
 // tile spills (444 us for 358).  A wave looks up one page a tile: four look-ups a wave
 // were as many scalar instructions as vector ones, 6% of the time.  Measured and not
 // kept: fixed interleaving of matrix and vector instructions (750 for 700 us), raised
 // priority of the waves in the first product (within 2%), values loaded only after the
-// keys are staged (spills).
+// keys are staged (spills), eight waves to a 64-row tile (500 tokens 27.4 for 27.6 us,
+// BF16 16.6 for 15.8), a term of the weights at a time over four blocks of the head
+// (30.7 for 27.6: spills), q's third term in the LDS for heads of 128 too (the same).
 template <uint32_t R, uint32_t C, int D, int KS>
 struct TileCfg {
     static constexpr int QT = kTerms<R>, KT = kTerms<C>, BM = 128 / KS;
