@@ -1223,7 +1223,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots, u
 // tokens, 32 heads on 4 of 128: 605-618 us, 890-910 TFLOP/s of the visible products,
 // where a large bf16 product reaches 1,220; packed prompts of f32 rows 339-345 us, 345
 // TFLOP/s and three times that in products; 777 tokens on 20,000 cached in E4M3 305 us,
-// 850 TFLOP/s.  A short prompt (500 tokens of f32 rows, 28 us) is 4 us to find its
+// 850 TFLOP/s.  A short prompt (500 tokens of f32 rows, 29 us) is 4 us to find its
 // tile, 8 to the end of the first 64 keys and 2 to 4 for each 64 after.
 //
 // 64-key tiles but where registers or LDS are short: with three terms of q a 64-key
@@ -1231,7 +1231,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs A, uint32_t slots, u
 // were as many scalar instructions as vector ones, 6% of the time.  Measured and not
 // kept: fixed interleaving of matrix and vector instructions (750 for 700 us), raised
 // priority of the waves in the first product (within 2%), values loaded only after the
-// keys are staged (spills), eight waves to a 64-row tile (500 tokens 27.4 for 27.6 us,
+// keys are staged (spills), eight waves to a 64-row tile (500 tokens of f32 rows 27.4 for 27.6 us,
 // BF16 16.6 for 15.8), a term of the weights at a time over four blocks of the head
 // (30.7 for 27.6: spills), q's third term in the LDS for heads of 128 too (the same).
 template <uint32_t R, uint32_t C, int D, int KS>

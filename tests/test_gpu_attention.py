@@ -146,6 +146,41 @@ def test_append_padding_rows(dev):
     assert not np.isnan(q[0]).any() and not np.isnan(q[2]).any()
 
 
+def test_append_norm_alone_first_rows_and_no_scales(dev):
+    """A norm of k alone without a rotation, sequences that start behind row 0
+    (the rows before them stay), an E4M3 cache without scales."""
+    say("append: k's norm alone, rows before the first sequence, no scales")
+    p = H.Problem("f32", "e4m3", (4, 2, 64), [3, 2], [3, 20], seed=9, dims=0, extra_rows=4)
+    p.upload(dev)
+    p.scale[:] = 1.0
+    p.cache.k_scale = p.cache.v_scale = None
+    p.drow0.upload(p.row0 + 4)
+    dk, dv, kn = dev.put(p.kx), dev.put(p.vx), dev.put(p.k_norm)
+    rot = attn.Rotation(None, 0, 0, k_norm=kn.ptr, eps=p.eps)
+    k0 = p.k.copy()
+    attn.append(p.cache, p.batch, "f32", p.dq.ptr, dk.ptr, dv.ptr, p.dout.ptr, p.hq, rot)
+    assert _lib.hip().colizig_hip_sync() == 0
+    q, k = p.dout.download(np.empty_like(p.out0)), p.dk.download(np.empty_like(p.k))
+    assert np.array_equal(q[:4].view(np.uint32), p.out0[:4].view(np.uint32))
+    assert np.array_equal(q[4:9], p.q[4:9])
+    for b in range(2):
+        r, n, L = p.row0[b] + 4, p.new[b], p.len[b]
+        x = p.kx[r:r + n].reshape(n, 2, 64).astype(np.float64)
+        ref, err = _turned(p, x, p.k_norm, None)
+        assert _held_ok(H.decode(p.get(k, b, L)[L - n:], "e4m3"), ref, err, "e4m3").all()
+        assert np.array_equal(p.get(k, b, L)[:L - n], p.get(k0, b, L)[:L - n])
+    p.k, p.v = k, p.dv.download(np.empty_like(p.v))
+    p.row0 = p.row0 + 4
+    p.scale_qk = 0.125
+    size = attn.work_bytes(p.cache, p.batch, p.hq)
+    work = dev.put(np.zeros(size, np.uint8))
+    p.dout.upload(p.out0)
+    attn.prompt(p.cache, p.batch, "f32", p.dq.ptr, p.dout.ptr, p.hq, 0.125, work.ptr, size)
+    got = p.fetch()
+    assert np.array_equal(got[:4].view(np.uint32), p.out0[:4].view(np.uint32))
+    p.check(got, rows=set(range(4, 9)))
+
+
 # ---- one token ------------------------------------------------------------------
 @pytest.mark.parametrize("rows,cache", TYPES)
 @pytest.mark.parametrize("heads,page,layout,pad,lens", [
