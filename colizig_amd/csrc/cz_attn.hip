@@ -5,8 +5,6 @@
 // at position len - new + i and sees the positions up to its own.
 #include "cz_attn.h"
 
-#include "cz_device.h"
-
 #include <algorithm>
 #include <type_traits>
 
@@ -148,13 +146,6 @@ struct Eight<kBF16> {
         }
     }
     __device__ __forceinline__ void terms(bf8 (&t)[1]) const { t[0] = __builtin_bit_cast(bf8, a); }
-};
-template <>
-struct Eight<kE4M3> {
-    u32x2 a;
-    __device__ __forceinline__ void load(const uint8_t *p) { a = *(const u32x2 *)p; }
-    __device__ __forceinline__ void zero() { a = u32x2{0, 0}; }
-    __device__ __forceinline__ void terms(bf8 (&t)[1]) const { t[0] = e4m3x8(a[0], a[1]); }
 };
 
 // threadIdx.x as a value that the compiler knows nothing of: what rare or final code
